@@ -41,28 +41,28 @@ def _loss(name, rows, d, vocab, grad, out, pad, bias):
 def listed():
     return [
         # the test model's 26 tensors: the call's latency
-        _adam("adam tiny, f32", 64, 256, 2, 256, "f32", 1, False),
+        _adam("adam tiny f32", 64, 256, 2, 256, "f32", 1, False),
         # nothing divides anything: tensors begin and end inside blocks and tiles; E4M3 gradients with scales
-        _adam("adam ragged, fp8", 333, 1001, 3, 10007, "fp8", 12345, True),
+        _adam("adam ragged fp8", 333, 1001, 3, 10007, "fp8", 12345, True),
         # the 185M model, float gradients as its training run has them, and bf16 ones
-        _adam("adam 185m, f32", 1024, 4096, 12, 16384, "f32", 100, True),
-        _adam("adam 185m, bf16", 1024, 4096, 12, 16384, "bf16", 2000, False),
+        _adam("adam 185m f32", 1024, 4096, 12, 16384, "f32", 100, True),
+        _adam("adam 185m bf16", 1024, 4096, 12, 16384, "bf16", 2000, False),
         # one token scored while a model is compared or sampled from: latency, the weights are read once
-        _loss("loss 185m, one token", 1, 1024, 16384, False, "f32", 0.0, True),
+        _loss("loss 185m one token", 1, 1024, 16384, False, "f32", 0.0, True),
         # a held-out text at an odd vocabulary, rows that are not 16-byte aligned
         _loss("loss ragged", 517, 712, 50257, False, "f32", 0.3, False),
         # one context of the 555M model evaluated
-        _loss("loss 555m, 2048 tokens", 2048, 1536, 100000, False, "f32", 0.0, True),
+        _loss("loss 555m 2048 tokens", 2048, 1536, 100000, False, "f32", 0.0, True),
         # the test model's training step
-        _loss("grad tiny, f32", 254, 64, 256, True, "f32", 0.0, True),
+        _loss("grad tiny f32", 254, 64, 256, True, "f32", 0.0, True),
         # packed short documents, over half of the rows are padding, odd everything
-        _loss("grad ragged, f32", 777, 331, 10007, True, "f32", 0.55, True),
+        _loss("grad ragged f32", 777, 331, 10007, True, "f32", 0.55, True),
         # a 4096-token microbatch of the 185M model into a float gradient flat
-        _loss("grad 185m, f32", 4096, 1024, 16384, True, "f32", 0.0, True),
+        _loss("grad 185m f32", 4096, 1024, 16384, True, "f32", 0.0, True),
         # a short fine-tuning batch of the 555M model: few rows, large vocabulary, bf16 gradients
-        _loss("grad 555m, 96 tokens, bf16", 96, 1536, 100000, True, "bf16", 0.1, True),
+        _loss("grad 555m 96 tokens bf16", 96, 1536, 100000, True, "bf16", 0.1, True),
         # a 4096-token microbatch of the 555M model into a bf16 gradient flat
-        _loss("grad 555m, bf16", 4096, 1536, 100000, True, "bf16", 0.0, True),
+        _loss("grad 555m bf16", 4096, 1536, 100000, True, "bf16", 0.0, True),
     ]
 
 
