@@ -36,6 +36,22 @@ static size_t round_up(size_t x, size_t a)
 	return (x + a - 1) / a * a;
 }
 
+/*
+** One moment flat.  8-bit moments: whole blocks of codes, one byte per element, then the blocks'
+** exponent bytes, so that whoever moves the flat as bytes moves both.
+*/
+static size_t moment_blocks(int64_t n)
+{
+	return ((size_t)n + kQ8Block - 1) / kQ8Block;
+}
+
+static size_t moment_bytes(int64_t n, int type)
+{
+	if (type == ANNI_Q8)
+		return moment_blocks(n) * (kQ8Block + 1);
+	return (size_t)n * elem_bytes(type);
+}
+
 /* Byte sizes of the flats of one arena. */
 struct Sizes {
 	int64_t	n;
@@ -314,7 +330,7 @@ static anni_adam *create_body(const anni_tensor *tensors, int n_tensors,
 		return nullptr;
 	(void)release_idle_pools();	/* the search for the arena's second half looks at what is free */
 	if (cfg->grad_type < ANNI_F32 || cfg->grad_type > ANNI_FP8_E4M3
-	    || (cfg->moment_type != ANNI_F32 && cfg->moment_type != ANNI_BF16)
+	    || (cfg->moment_type != ANNI_F32 && cfg->moment_type != ANNI_BF16 && cfg->moment_type != ANNI_Q8)
 	    || cfg->grad_slots < 0 || cfg->grad_slots > 4096
 	    || cfg->layout < ANNI_LAYOUT_AUTO || cfg->layout > ANNI_LAYOUT_SPLIT)
 		return nullptr;
@@ -366,7 +382,7 @@ static anni_adam *create_body(const anni_tensor *tensors, int n_tensors,
 	z.n_tiles = (n + kTile - 1) / kTile;
 	z.n_slots = cfg->grad_slots;
 	z.p_bytes = (size_t)n * 4;
-	z.mv_bytes = (size_t)n * elem_bytes(cfg->moment_type);
+	z.mv_bytes = moment_bytes(n, cfg->moment_type);
 	z.tw_bytes = cfg->twins ? (size_t)n * 2 : 0;
 	z.g_bytes = round_up((size_t)n * elem_bytes(cfg->grad_type), big);
 	pv->z = z;
@@ -801,6 +817,10 @@ static void describe(const anni_adam *opt, Flat *f)
 	f->n = opt->n;
 	f->grad_type = opt->cfg.grad_type;
 	f->moment_type = opt->cfg.moment_type;
+	if (f->moment_type == ANNI_Q8 && f->m && f->v) {
+		f->m_exp = (uint8_t *)f->m + moment_blocks(opt->n) * kQ8Block;
+		f->v_exp = (uint8_t *)f->v + moment_blocks(opt->n) * kQ8Block;
+	}
 	f->segs = pv->d_segs;
 	f->tile_seg = pv->d_tile_seg;
 	f->gscale = opt->d_gscale;
@@ -1069,6 +1089,7 @@ static int step_impl(anni_adam *opt, double lr, double grad_scale, hipEvent_t *e
 	c.lr = lr;
 	c.decay_on = opt->weight_decay > 0.0 ? 1 : 0;	/* lm_adam.c:594 */
 	c.lr_wd = c.decay_on ? lr * opt->weight_decay : 0.0;
+	c.dither = dither_seed((uint32_t)t);
 	describe(opt, &f);
 	memset(&norm, 0, sizeof(norm));
 	/* lm_adam.c:466: the norm is wanted for the clip, for the skip, or just to be printed */
@@ -1232,6 +1253,26 @@ struct PairIo {
 static int write_all(int fd, const void *buf, size_t n);
 static int read_all(int fd, void *buf, size_t n);
 
+static int pairs_out(const anni_adam *opt, hipStream_t st, float *pairs, int64_t first, int64_t count)
+{
+	Flat f;
+
+	if (opt->cfg.moment_type != ANNI_Q8)
+		return launch_mv_interleave(st, pairs, opt->d_m, opt->d_v, opt->cfg.moment_type, first, count);
+	describe(opt, &f);
+	return launch_mv_interleave_q8(st, pairs, f, first, count);
+}
+
+static int pairs_in(const anni_adam *opt, hipStream_t st, const float *pairs, int64_t first, int64_t count)
+{
+	Flat f;
+
+	if (opt->cfg.moment_type != ANNI_Q8)
+		return launch_mv_deinterleave(st, opt->d_m, opt->d_v, opt->cfg.moment_type, pairs, first, count);
+	describe(opt, &f);
+	return launch_mv_deinterleave_q8(st, f, pairs, first, count);
+}
+
 /*
 ** Slots [first, first + count) as (m, v) pairs, chunk by chunk: while the host consumes chunk k
 ** out of one page-locked buffer (a copy into the caller's array, or write(2) straight from the
@@ -1254,8 +1295,7 @@ static int export_pairs(anni_adam *opt, int64_t first, int64_t count, const Pair
 			const int64_t c = count - at < kCkptChunk ? count - at : kCkptChunk;
 			const int b = (int)((k + 1) & 1);
 
-			if (launch_mv_interleave(st, sg.dev[b], opt->d_m, opt->d_v, opt->cfg.moment_type,
-			    first + at, c) != 0
+			if (pairs_out(opt, st, sg.dev[b], first + at, c) != 0
 			    || !hip_ok(hipMemcpyAsync(sg.host[b], sg.dev[b], (size_t)c * 2 * sizeof(float),
 			    hipMemcpyDeviceToHost, st), "export d2h")
 			    || !hip_ok(hipEventRecord(sg.ev[b], st), "export event")) {
@@ -1296,8 +1336,11 @@ static int import_pairs(anni_adam *opt, int64_t first, int64_t count, const Pair
 	if (!sg.init())
 		return -1;
 	st = compute_stream();
-	for (int64_t at = 0, k = 0; at < count && rc == 0; at += kCkptChunk, k++) {
-		const int64_t c = count - at < kCkptChunk ? count - at : kCkptChunk;
+	for (int64_t at = 0, k = 0, c; at < count && rc == 0; at += c, k++) {
+		/* every chunk but the last ends where a block of 8-bit moments does: no block is encoded twice */
+		c = kCkptChunk - (first + at) % kQ8Block;
+		if (count - at < c)
+			c = count - at;
 		const int b = (int)(k & 1);
 		const size_t bytes = (size_t)c * 2 * sizeof(float);
 
@@ -1312,8 +1355,7 @@ static int import_pairs(anni_adam *opt, int64_t first, int64_t count, const Pair
 		}
 		if (rc == 0 && (!hip_ok(hipMemcpyAsync(sg.dev[b], sg.host[b], bytes, hipMemcpyHostToDevice,
 		    st), "import h2d")
-		    || launch_mv_deinterleave(st, opt->d_m, opt->d_v, opt->cfg.moment_type, sg.dev[b],
-		    first + at, c) != 0
+		    || pairs_in(opt, st, sg.dev[b], first + at, c) != 0
 		    || !hip_ok(hipEventRecord(sg.ev[b], st), "import event")))
 			rc = -1;
 	}
@@ -1344,6 +1386,24 @@ int anni_adam_import_mv(anni_adam *opt, int64_t first, int64_t count, const floa
 	io.mem = const_cast<float *>(pairs);
 	io.fd = -1;
 	return with_moments(opt, [&] { return import_pairs(opt, first, count, io); });
+}
+
+int anni_adam_read_moments(anni_adam *opt, int64_t first, int64_t count, int type, void *d_m, void *d_v)
+{
+	if (!opt || !opt->priv || (!d_m && !d_v) || first < 0 || count < 0 || first > opt->n
+	    || count > opt->n - first || (type != ANNI_F32 && type != ANNI_BF16) || !device_ready())
+		return -1;
+	/* an element starts where its type may */
+	if ((((uintptr_t)d_m | (uintptr_t)d_v) & (elem_bytes(type) - 1)) != 0)
+		return -1;
+	if (count == 0)
+		return 0;
+	return with_moments(opt, [&] {
+		Flat f;
+
+		describe(opt, &f);
+		return launch_read_moments(compute_stream(), f, first, count, type, d_m, d_v);
+	});
 }
 
 static int write_all(int fd, const void *buf, size_t n)

@@ -22,7 +22,7 @@
 
 namespace anni {
 
-enum { kF32 = 0, kBF16 = 1, kFP8 = 2 };
+enum { kF32 = 0, kBF16 = 1, kFP8 = 2, kQ8 = 3 };	/* kQ8: moments only */
 
 constexpr int kThreads = 256;			/* four 64-lane wavefronts */
 constexpr int kQuad = 4;			/* elements per lane per access */
@@ -84,6 +84,8 @@ struct Flat {
 	void		*g;
 	void		*m;
 	void		*v;
+	uint8_t		*m_exp;		/* 8-bit moments: the exponent byte of every block of kQ8Block elements */
+	uint8_t		*v_exp;
 	uint16_t	*twin;		/* may be NULL */
 	int64_t		n;
 	int		grad_type;
@@ -204,6 +206,16 @@ int	launch_mv_interleave(hipStream_t st, float *pairs, const void *m, const void
 /* The inverse: m[first+k] = pairs[2k], v[first+k] = pairs[2k+1] (bf16 moments: round to nearest even). */
 int	launch_mv_deinterleave(hipStream_t st, void *m, void *v, int moment_type, const float *pairs,
 		int64_t first, int64_t count);
+/*
+** The same two for 8-bit moments (n elements in all).  An import rounds to nearest and gives every
+** block it touches a new exponent: the block's other elements are decoded and encoded with it.
+*/
+int	launch_mv_interleave_q8(hipStream_t st, float *pairs, const Flat &f, int64_t first, int64_t count);
+int	launch_mv_deinterleave_q8(hipStream_t st, const Flat &f, const float *pairs, int64_t first,
+		int64_t count);
+/* dm[k] = m[first + k], dv[k] = v[first + k] as kF32 or kBF16 values; either destination may be NULL. */
+int	launch_read_moments(hipStream_t st, const Flat &f, int64_t first, int64_t count, int type,
+		void *dm, void *dv);
 int	launch_fill_bytes(hipStream_t st, void *dst, int value, size_t nbytes);
 
 } /* namespace anni */

@@ -59,6 +59,7 @@ template <int T> struct RawQuad;
 template <> struct RawQuad<kF32> { f32x4 v; };
 template <> struct RawQuad<kBF16> { u32x2 v; };
 template <> struct RawQuad<kFP8> { uint32_t v; };
+template <> struct RawQuad<kQ8> { uint32_t v; };
 
 template <int T, bool NT>
 __device__ __forceinline__ RawQuad<T> load_raw(const void *base, int64_t i)
@@ -783,6 +784,8 @@ struct UpdateArgs {
 	void		*m;
 	void		*v;
 	uint16_t	*twin;
+	uint8_t		*m_exp;		/* 8-bit moments */
+	uint8_t		*v_exp;
 	int64_t		n;
 	const Seg	*segs;
 	const int32_t	*tile_seg;
@@ -987,6 +990,164 @@ __global__ __launch_bounds__(kThreads) void adam_update_kernel(UpdateArgs a)
 ** Arithmetic, rounding points and stores are those of adam_update_kernel; results are
 ** bit-identical.
 */
+/* ---- 8-bit moments ------------------------------------------------------------ */
+
+/*
+** The largest of the 64 lanes' words, each half on its own as 16-bit unsigned numbers: four DPP
+** shifts inside the rows of 16 lanes, two broadcasts between rows; no LDS.  Uniform result.
+*/
+__device__ __forceinline__ uint32_t wave_max_pair(uint32_t x)
+{
+	typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+#define ANNI_MAX_STEP(ctrl, rows) \
+	x = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), \
+	    __builtin_bit_cast(u16x2, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, rows, 0xf, false))))
+
+	ANNI_MAX_STEP(0x111, 0xf);	/* row_shr 1, 2, 4, 8 */
+	ANNI_MAX_STEP(0x112, 0xf);
+	ANNI_MAX_STEP(0x114, 0xf);
+	ANNI_MAX_STEP(0x118, 0xf);
+	ANNI_MAX_STEP(0x142, 0xa);	/* row_bcast 15 into rows 1 and 3 */
+	ANNI_MAX_STEP(0x143, 0xc);	/* row_bcast 31 into rows 2 and 3 */
+#undef ANNI_MAX_STEP
+	return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+/* Four moments of a lane from their codes; b_m and b_v are the block's exponent bytes (uniform). */
+__device__ __forceinline__ void q8_widen(uint32_t cm, uint32_t cv, uint32_t b_m, uint32_t b_v, f32x4 &M,
+	f32x4 &V)
+{
+	const f32x2_t lo = fp8_e4m3_decode2(cm, false);
+	const f32x2_t hi = fp8_e4m3_decode2(cm, true);
+	const int km = q8_top(b_m) - 8;
+	const int kv = q8_top(b_v) + 96;
+
+	M.x = __builtin_ldexpf(lo.x, km);
+	M.y = __builtin_ldexpf(lo.y, km);
+	M.z = __builtin_ldexpf(hi.x, km);
+	M.w = __builtin_ldexpf(hi.y, km);
+	V.x = __builtin_ldexpf(__uint_as_float((cv << 20) & 0x0ff00000u), kv);
+	V.y = __builtin_ldexpf(__uint_as_float((cv << 12) & 0x0ff00000u), kv);
+	V.z = __builtin_ldexpf(__uint_as_float((cv << 4) & 0x0ff00000u), kv);
+	V.w = __builtin_ldexpf(__uint_as_float((cv >> 4) & 0x0ff00000u), kv);
+	if (b_m == 255u)
+		M = f32x4{1.0f, 1.0f, 1.0f, 1.0f} * __uint_as_float(0x7fc00000u);
+	if (b_v == 255u)
+		V = f32x4{1.0f, 1.0f, 1.0f, 1.0f} * __uint_as_float(0x7fc00000u);
+}
+
+/* The largest |x| of four values as bits (a NaN is larger than any number). */
+__device__ __forceinline__ uint32_t amax4_bits(f32x4 x)
+{
+	uint32_t r = 0u;
+
+#pragma unroll
+	for (int k = 0; k < kQuad; k++) {
+		const uint32_t u = __float_as_uint(x[k]) & 0x7fffffffu;
+
+		r = r > u ? r : u;
+	}
+	return r;
+}
+
+/*
+** New moments of a block, four per lane: its exponents over the wavefront, then the codes.  x0 is
+** the place of the lane's first element times kDitherGold, plus the step's seed.
+*/
+struct Q8Block {
+	uint32_t	cm, cv;		/* four codes each */
+	uint32_t	b_m, b_v;
+};
+
+__device__ __forceinline__ Q8Block q8_narrow(f32x4 M, f32x4 V, uint32_t x0)
+{
+	const uint32_t both = wave_max_pair(q8_exponent(amax4_bits(M)) | (q8_exponent(amax4_bits(V)) << 16));
+	Q8Block r;
+
+	r.b_m = both & 0xffffu;
+	r.b_v = both >> 16;
+	r.cm = 0u;
+	r.cv = 0u;
+#pragma unroll
+	for (int k = 0; k < kQuad; k++) {
+		const uint32_t z = dither_bits(x0 + (uint32_t)k * kDitherGold);
+
+		r.cm |= q8_code_m(M[k], q8_top(r.b_m), (z & 0xffffu) << 4) << (8 * k);
+		r.cv |= q8_code_v(V[k], q8_top(r.b_v), (z >> 12) & 0xffff0u) << (8 * k);
+	}
+	/* a block that is not finite keeps no codes (they would not fit their bytes) */
+	if (r.b_m == 255u)
+		r.cm = 0u;
+	if (r.b_v == 255u)
+		r.cv = 0u;
+	return r;
+}
+
+/*
+** A tile on the element-wise path with 8-bit moments: still a block per wavefront, four elements to
+** a lane, because the block's exponent needs all of them.  Elements behind the flat count as 0.
+*/
+template <int GT, bool DER>
+__device__ __forceinline__ void tile_slow_q8(const UpdateArgs &a, const TileInfo &t, double gs, int tid)
+{
+	for (int u = 0; u < kQuadsPerTile; u++) {
+		const int64_t i0 = t.base + (int64_t)(u * kThreads + tid) * kQuad;
+		const int64_t blk = i0 / kQ8Block;
+		f32x4 M = {0.0f, 0.0f, 0.0f, 0.0f}, V = M;
+		int s = t.s;
+
+		if (t.base + (int64_t)(u * kThreads + (tid & ~63)) * kQuad >= t.end)
+			return;			/* the whole block lies behind the flat; the same in every lane */
+		q8_widen(*(const uint32_t *)((const uint8_t *)a.m + i0), *(const uint32_t *)((const uint8_t *)a.v + i0),
+		    (uint32_t)__builtin_amdgcn_readfirstlane(a.m_exp[blk]),
+		    (uint32_t)__builtin_amdgcn_readfirstlane(a.v_exp[blk]), M, V);
+#pragma unroll
+		for (int k = 0; k < kQuad; k++) {
+			const int64_t i = i0 + k;
+			uint32_t flags = a.uniform_flags;
+			float sc = 1.0f;
+
+			if (i >= t.end) {
+				M[k] = 0.0f;
+				V[k] = 0.0f;
+				continue;
+			}
+			if (a.segs) {
+				while (i >= a.segs[s].end)
+					s++;
+				flags = a.segs[s].flags;
+			}
+			if (GT == kFP8)
+				sc = a.gscale[s];
+			const Elem e = adam_elem<true>(a.p[i], load_one<GT>(a.g, i, sc), M[k], V[k], gs, a.c,
+			    a.c.decay_on && (flags & kSegDecay) != 0);
+
+			M[k] = e.m;
+			V[k] = e.v;
+			a.p[i] = e.p;
+			zero_one<GT>(a.g, i);
+			if ((flags & kSegTwin) != 0 && a.twin != nullptr)
+				a.twin[i] = (uint16_t)bf16_rne(e.p);
+			if (DER && (flags & kSegFp8Twin) != 0 && a.der.wamax != nullptr) {
+				const float ab = fmaxf(0.0f, fabsf(e.p));
+
+				if (ab > 0.0f)
+					amax_raise(a.der.wamax + s, ab);
+			}
+			if (DER && (flags & kSegPack) != 0 && a.der.pack != nullptr)
+				pack_one(a.der.pack, a.der.packs[s], (uint32_t)(i - a.segs[s].begin), e.p);
+		}
+		const Q8Block b = q8_narrow(M, V, (uint32_t)i0 * kDitherGold + a.c.dither);
+
+		*(uint32_t *)((uint8_t *)a.m + i0) = b.cm;
+		*(uint32_t *)((uint8_t *)a.v + i0) = b.cv;
+		if ((tid & 63) == 0) {
+			a.m_exp[blk] = (uint8_t)b.b_m;
+			a.v_exp[blk] = (uint8_t)b.b_v;
+		}
+	}
+}
+
 /* A tile that is skipped, ragged or shared by several tensors: as in adam_update_kernel. */
 template <int GT, int MT, bool NT, bool DER>
 __device__ __forceinline__ void tile_slow(const UpdateArgs &a, const TileInfo &t, double gs,
@@ -1005,6 +1166,9 @@ __device__ __forceinline__ void tile_slow(const UpdateArgs &a, const TileInfo &t
 		}
 		return;
 	}
+	if constexpr (MT == kQ8) {
+		tile_slow_q8<GT, DER>(a, t, gs, tid);
+	} else {
 	for (int64_t i = t.base + tid; i < t.end; i += kThreads) {
 		uint32_t flags = a.uniform_flags;
 		float sc = 1.0f;
@@ -1035,6 +1199,7 @@ __device__ __forceinline__ void tile_slow(const UpdateArgs &a, const TileInfo &t
 		if (DER && (flags & kSegPack) != 0 && a.der.pack != nullptr)
 			pack_one(a.der.pack, a.der.packs[s], (uint32_t)(i - a.segs[s].begin), e.p);
 	}
+	}
 }
 
 template <int GT, int MT>
@@ -1043,6 +1208,8 @@ struct HalfStage {
 	RawQuad<GT>	G[kQuadsPerTile / 2];
 	RawQuad<MT>	M[kQuadsPerTile / 2];
 	RawQuad<MT>	V[kQuadsPerTile / 2];
+	uint32_t	EM[kQuadsPerTile / 2];	/* 8-bit moments: the exponent bytes of the quad's block */
+	uint32_t	EV[kQuadsPerTile / 2];
 };
 
 template <int GT, int MT, bool NT, int Q0>
@@ -1057,6 +1224,10 @@ __device__ __forceinline__ void half_load(HalfStage<GT, MT> &st, const UpdateArg
 		st.M[u] = load_raw<MT, NT>(a.m, idx);
 		st.V[u] = load_raw<MT, NT>(a.v, idx);
 		st.P[u] = ld<NT>((const f32x4 *)(a.p + idx));
+		if constexpr (MT == kQ8) {
+			st.EM[u] = a.m_exp[idx / kQ8Block];
+			st.EV[u] = a.v_exp[idx / kQ8Block];
+		}
 	}
 }
 
@@ -1082,9 +1253,17 @@ __device__ __forceinline__ void half_consume(const HalfStage<GT, MT> &st, const 
 	for (int u = 0; u < kQuadsPerTile / 2; u++) {
 		const int64_t idx = t.base + (int64_t)((Q0 + u) * kThreads + tid) * kQuad;
 		const f32x4 G = widen_raw<GT>(st.G[u], sc);
-		f32x4 M = widen_raw<MT>(st.M[u], 1.0f);
-		f32x4 V = widen_raw<MT>(st.V[u], 1.0f);
+		f32x4 M, V;
 		f32x4 P = st.P[u];
+
+		if constexpr (MT == kQ8) {
+			/* the 64 lanes of a quad access hold exactly one block: its exponents are uniform */
+			q8_widen(st.M[u].v, st.V[u].v, (uint32_t)__builtin_amdgcn_readfirstlane((int)st.EM[u]),
+			    (uint32_t)__builtin_amdgcn_readfirstlane((int)st.EV[u]), M, V);
+		} else {
+			M = widen_raw<MT>(st.M[u], 1.0f);
+			V = widen_raw<MT>(st.V[u], 1.0f);
+		}
 
 #pragma unroll
 		for (int k = 0; k < kQuad; k++) {
@@ -1096,8 +1275,19 @@ __device__ __forceinline__ void half_consume(const HalfStage<GT, MT> &st, const 
 			V[k] = e.v;
 		}
 		store_quad<kF32, NT>(a.p, idx, P);
-		store_quad<MT, NT>(a.m, idx, M);
-		store_quad<MT, NT>(a.v, idx, V);
+		if constexpr (MT == kQ8) {
+			const Q8Block b = q8_narrow(M, V, (uint32_t)idx * kDitherGold + a.c.dither);
+
+			anni::st<NT>((uint32_t *)((uint8_t *)a.m + idx), b.cm);
+			anni::st<NT>((uint32_t *)((uint8_t *)a.v + idx), b.cv);
+			if ((tid & 63) == 0) {
+				a.m_exp[idx / kQ8Block] = (uint8_t)b.b_m;
+				a.v_exp[idx / kQ8Block] = (uint8_t)b.b_v;
+			}
+		} else {
+			store_quad<MT, NT>(a.m, idx, M);
+			store_quad<MT, NT>(a.v, idx, V);
+		}
 		zero_quad<GT, NT>(a.g, idx);
 		if (twin)
 			store_quad<kBF16, NT>(a.twin, idx, P);
@@ -1416,6 +1606,163 @@ __global__ __launch_bounds__(kThreads) void mv_deinterleave_kernel(void *m, void
 	}
 }
 
+/* ---- 8-bit moments in and out ---------------------------------------------------- */
+
+struct MomentArgs {
+	const void	*m;
+	const void	*v;
+	const uint8_t	*m_exp;
+	const uint8_t	*v_exp;
+	int64_t		first;
+	int64_t		count;
+	void		*dm;
+	void		*dv;
+	int		vec_ok;		/* eight elements at a time: sources and destinations allow 8- and 16-byte accesses */
+};
+
+template <int MT>
+__device__ __forceinline__ float moment_one(const void *x, const uint8_t *ex, int64_t i, bool second)
+{
+	if constexpr (MT == kQ8) {
+		const uint32_t c = ((const uint8_t *)x)[i];
+		const uint32_t b = ex[i / kQ8Block];
+
+		return second ? q8_value_v(c, b) : q8_value_m(c, b);
+	} else {
+		return load_one<MT>(x, i, 1.0f);
+	}
+}
+
+/* Eight moments from element i (i % 8 == 0) as floats. */
+template <int MT>
+__device__ __forceinline__ void moment_eight(const void *x, const uint8_t *ex, int64_t i, bool second,
+	f32x4 (&r)[2])
+{
+	if constexpr (MT == kQ8) {
+		const u32x2 c = ld<true>((const u32x2 *)((const uint8_t *)x + i));
+		const uint32_t b = ex[i / kQ8Block];
+
+#pragma unroll
+		for (int h = 0; h < 2; h++)
+#pragma unroll
+			for (int k = 0; k < kQuad; k++) {
+				const uint32_t one = (c[h] >> (8 * k)) & 0xffu;
+
+				r[h][k] = second ? q8_value_v(one, b) : q8_value_m(one, b);
+			}
+	} else {
+		r[0] = load_quad<MT, true>(x, i, 1.0f);
+		r[1] = load_quad<MT, true>(x, i + kQuad, 1.0f);
+	}
+}
+
+template <int OT>
+__device__ __forceinline__ void store_eight(void *dst, int64_t k, const f32x4 (&r)[2])
+{
+	typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+	if constexpr (OT == kF32) {
+		store_quad<kF32, true>(dst, k, r[0]);
+		store_quad<kF32, true>(dst, k + kQuad, r[1]);
+	} else {
+		const u32x4 w = {bf16_rne2(r[0].x, r[0].y), bf16_rne2(r[0].z, r[0].w), bf16_rne2(r[1].x, r[1].y),
+		    bf16_rne2(r[1].z, r[1].w)};
+
+		st<true>((u32x4 *)((uint16_t *)dst + k), w);
+	}
+}
+
+/* A stream: eight elements per lane and access, m and v of four such places in flight. */
+template <int MT, int OT>
+__global__ __launch_bounds__(kThreads) void read_moments_kernel(MomentArgs a)
+{
+	const int64_t stride = (int64_t)gridDim.x * kThreads;
+	const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+	const int64_t n8 = a.vec_ok ? a.count / 8 : 0;
+
+#pragma unroll 4
+	for (int64_t q = at; q < n8; q += stride) {
+		f32x4 r[2];
+
+		if (a.dm) {
+			moment_eight<MT>(a.m, a.m_exp, a.first + q * 8, false, r);
+			store_eight<OT>(a.dm, q * 8, r);
+		}
+		if (a.dv) {
+			moment_eight<MT>(a.v, a.v_exp, a.first + q * 8, true, r);
+			store_eight<OT>(a.dv, q * 8, r);
+		}
+	}
+	for (int64_t k = n8 * 8 + at; k < a.count; k += stride) {
+		if (a.dm)
+			store_one<OT>(a.dm, k, moment_one<MT>(a.m, a.m_exp, a.first + k, false));
+		if (a.dv)
+			store_one<OT>(a.dv, k, moment_one<MT>(a.v, a.v_exp, a.first + k, true));
+	}
+}
+
+__global__ __launch_bounds__(kThreads) void mv_interleave_q8_kernel(float *pairs, MomentArgs a)
+{
+	typedef float f32x2 __attribute__((ext_vector_type(2)));
+	const int64_t stride = (int64_t)gridDim.x * kThreads;
+
+	for (int64_t k = (int64_t)blockIdx.x * kThreads + threadIdx.x; k < a.count; k += stride) {
+		f32x2 mv;
+
+		mv.x = moment_one<kQ8>(a.m, a.m_exp, a.first + k, false);
+		mv.y = moment_one<kQ8>(a.v, a.v_exp, a.first + k, true);
+		*(f32x2 *)(pairs + 2 * k) = mv;
+	}
+}
+
+/* One wavefront per block that [first, first + count) touches, four elements per lane. */
+__global__ __launch_bounds__(kThreads) void mv_deinterleave_q8_kernel(uint8_t *m, uint8_t *v, uint8_t *m_exp,
+	uint8_t *v_exp, int64_t n, const float *pairs, int64_t first, int64_t count)
+{
+	const int64_t b0 = first / kQ8Block;
+	const int64_t b1 = (first + count - 1) / kQ8Block;
+	const int64_t step = (int64_t)gridDim.x * kWaves;
+
+	for (int64_t blk = b0 + (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); blk <= b1; blk += step) {
+		const int64_t i0 = blk * kQ8Block + (threadIdx.x & 63) * kQuad;
+		f32x4 M, V;
+		uint32_t cm = 0u, cv = 0u;
+
+		q8_widen(*(const uint32_t *)(m + i0), *(const uint32_t *)(v + i0),
+		    (uint32_t)__builtin_amdgcn_readfirstlane(m_exp[blk]),
+		    (uint32_t)__builtin_amdgcn_readfirstlane(v_exp[blk]), M, V);
+#pragma unroll
+		for (int k = 0; k < kQuad; k++) {
+			const int64_t at = i0 + k - first;
+
+			if (at >= 0 && at < count) {
+				M[k] = pairs[2 * at];
+				V[k] = pairs[2 * at + 1];
+				if (V[k] < 0.0f)
+					V[k] = 0.0f;	/* the format has no sign */
+			} else if (i0 + k >= n) {
+				M[k] = 0.0f;
+				V[k] = 0.0f;
+			}
+		}
+		const uint32_t both = wave_max_pair(q8_exponent(amax4_bits(M)) | (q8_exponent(amax4_bits(V)) << 16));
+		const uint32_t b_m = both & 0xffffu;
+		const uint32_t b_v = both >> 16;
+
+#pragma unroll
+		for (int k = 0; k < kQuad; k++) {
+			cm |= q8_code_m(M[k], q8_top(b_m), q8_nearest(M[k], -112 - q8_top(b_m))) << (8 * k);
+			cv |= q8_code_v(V[k], q8_top(b_v), q8_nearest(V[k], -96 - q8_top(b_v))) << (8 * k);
+		}
+		*(uint32_t *)(m + i0) = b_m == 255u ? 0u : cm;
+		*(uint32_t *)(v + i0) = b_v == 255u ? 0u : cv;
+		if ((threadIdx.x & 63) == 0) {
+			m_exp[blk] = (uint8_t)b_m;
+			v_exp[blk] = (uint8_t)b_v;
+		}
+	}
+}
+
 /* Byte fill on the stream (a kernel, so it can sit in a captured graph). */
 __global__ __launch_bounds__(kThreads) void fill_bytes_kernel(uint8_t *dst, uint32_t pattern,
 	size_t nbytes, size_t head, size_t n16)
@@ -1572,7 +1919,10 @@ static int check_flat(const Flat &f, bool need_state)
 	if (need_state) {
 		if (!f.p || !f.m || !f.v)
 			return -1;
-		if (f.moment_type != kF32 && f.moment_type != kBF16)
+		if (f.moment_type != kF32 && f.moment_type != kBF16 && f.moment_type != kQ8)
+			return -1;
+		/* blocks of codes are read and written four at a time, also on the element-wise path */
+		if (f.moment_type == kQ8 && (!f.m_exp || !f.v_exp || !aligned(f.m, 4) || !aligned(f.v, 4)))
 			return -1;
 	}
 	return 0;
@@ -1945,7 +2295,8 @@ static void update_launch(hipStream_t st, int grid, const UpdateArgs &a)
 	constexpr bool narrow = GT != kF32 || MT != kF32;
 	const bool der = a.der.wamax != nullptr || a.der.pack != nullptr;
 
-	if (pipe_level() >= (narrow ? 1 : 2)) {
+	/* 8-bit moments have the pipelined kernel only: there a wavefront holds whole blocks */
+	if (MT == kQ8 || pipe_level() >= (narrow ? 1 : 2)) {
 		if (der) {
 			if (nt_on())
 				hipLaunchKernelGGL((adam_update_pipe_kernel<GT, MT, true, true>), dim3(grid),
@@ -1962,6 +2313,7 @@ static void update_launch(hipStream_t st, int grid, const UpdateArgs &a)
 		}
 		return;
 	}
+	if constexpr (MT != kQ8) {
 	if (der) {
 		if (nt_on())
 			hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, true, true>), dim3(grid),
@@ -1975,6 +2327,7 @@ static void update_launch(hipStream_t st, int grid, const UpdateArgs &a)
 	} else {
 		hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, false, false>), dim3(grid),
 		    dim3(kThreads), 0, st, a);
+	}
 	}
 }
 
@@ -2042,6 +2395,8 @@ static int update_go(hipStream_t st, const Flat &f, const StepConsts &c, double 
 	a.g = f.g;
 	a.m = f.m;
 	a.v = f.v;
+	a.m_exp = f.m_exp;
+	a.v_exp = f.v_exp;
 	a.twin = f.twin;
 	a.n = f.n;
 	a.segs = f.segs;
@@ -2066,6 +2421,13 @@ static int update_go(hipStream_t st, const Flat &f, const StepConsts &c, double 
 			update_launch<kBF16, kF32>(st, grid, a);
 		else
 			update_launch<kFP8, kF32>(st, grid, a);
+	} else if (f.moment_type == kQ8) {
+		if (f.grad_type == kF32)
+			update_launch<kF32, kQ8>(st, grid, a);
+		else if (f.grad_type == kBF16)
+			update_launch<kBF16, kQ8>(st, grid, a);
+		else
+			update_launch<kFP8, kQ8>(st, grid, a);
 	} else {
 		if (f.grad_type == kF32)
 			update_launch<kF32, kBF16>(st, grid, a);
@@ -2214,6 +2576,73 @@ int launch_mv_deinterleave(hipStream_t st, void *m, void *v, int moment_type, co
 		    dim3(kThreads), 0, st, m, v, pairs, first, count);
 	else
 		return -1;
+	return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+static MomentArgs moment_args(const Flat &f, int64_t first, int64_t count, void *dm, void *dv)
+{
+	MomentArgs a;
+
+	memset(&a, 0, sizeof(a));
+	a.m = f.m;
+	a.v = f.v;
+	a.m_exp = f.m_exp;
+	a.v_exp = f.v_exp;
+	a.first = first;
+	a.count = count;
+	a.dm = dm;
+	a.dv = dv;
+	return a;
+}
+
+int launch_mv_interleave_q8(hipStream_t st, float *pairs, const Flat &f, int64_t first, int64_t count)
+{
+	if (!pairs || !f.m || !f.v || !f.m_exp || !f.v_exp || f.moment_type != kQ8 || first < 0 || count <= 0
+	    || first + count > f.n)
+		return -1;
+	hipLaunchKernelGGL(mv_interleave_q8_kernel, dim3(helper_grid(count)), dim3(kThreads), 0, st, pairs,
+	    moment_args(f, first, count, nullptr, nullptr));
+	return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_mv_deinterleave_q8(hipStream_t st, const Flat &f, const float *pairs, int64_t first,
+	int64_t count)
+{
+	if (!pairs || !f.m || !f.v || !f.m_exp || !f.v_exp || f.moment_type != kQ8 || first < 0 || count <= 0
+	    || first + count > f.n)
+		return -1;
+	hipLaunchKernelGGL(mv_deinterleave_q8_kernel, dim3(helper_grid((count + kQuad - 1) / kQuad)),
+	    dim3(kThreads), 0, st, (uint8_t *)f.m, (uint8_t *)f.v, f.m_exp, f.v_exp, f.n, pairs, first, count);
+	return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+template <int MT>
+static void read_moments_launch(hipStream_t st, const MomentArgs &a, int type)
+{
+	const int grid = helper_grid((a.count + 7) / 8);
+
+	if (type == kF32)
+		hipLaunchKernelGGL((read_moments_kernel<MT, kF32>), dim3(grid), dim3(kThreads), 0, st, a);
+	else
+		hipLaunchKernelGGL((read_moments_kernel<MT, kBF16>), dim3(grid), dim3(kThreads), 0, st, a);
+}
+
+int launch_read_moments(hipStream_t st, const Flat &f, int64_t first, int64_t count, int type, void *dm,
+	void *dv)
+{
+	MomentArgs a = moment_args(f, first, count, dm, dv);
+
+	if ((!dm && !dv) || !f.m || !f.v || first < 0 || count <= 0 || first + count > f.n
+	    || (type != kF32 && type != kBF16) || (f.moment_type == kQ8 && (!f.m_exp || !f.v_exp)))
+		return -1;
+	a.vec_ok = first % 8 == 0 && (!dm || aligned(dm, 16)) && (!dv || aligned(dv, 16)) && aligned(f.m, 16)
+	    && aligned(f.v, 16) ? 1 : 0;
+	if (f.moment_type == kF32)
+		read_moments_launch<kF32>(st, a, type);
+	else if (f.moment_type == kBF16)
+		read_moments_launch<kBF16>(st, a, type);
+	else
+		read_moments_launch<kQ8>(st, a, type);
 	return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

@@ -30,6 +30,7 @@ struct StepConsts {
 	int	decay_on;	/* weight_decay > 0 (lm_adam.c:594); per-tensor flags select where */
 	double	rbc1;	/* 1.0 / bc1 and 1.0 / bc2, correctly rounded (host division) */
 	double	rbc2;
+	uint32_t dither;	/* dither_seed(t): 8-bit moments only */
 };
 
 /* New p, m, v of one element. */
@@ -226,6 +227,108 @@ __device__ __forceinline__ float scale_from_amax(float a)
 	if (a < 1e-12f)
 		a = 1e-12f;
 	return a;
+}
+
+/* ---- moments in 8 bits ------------------------------------------------------ */
+
+/*
+** A moment of ANNI_Q8 storage is a small float times a power of two shared by 256 neighbours of
+** the flat (kQ8Block).  The shared exponent is a byte B, E = max(B, 1) - 127: the least one with
+** max |x| <= 1.75 * 2^E.  Then
+**   m = OCP E4M3 code * 2^(E - 8)	sign, 15 normal binades below 2^E, 2^(E-17) the smallest step
+**   v = unsigned code of 5 exponent and 3 fraction bits: field f > 0 (1 + r/8) * 2^(E + f - 31),
+**       field 0 r * 2^(E - 33)
+** Both have eight steps to the binade; v needs twice the binades because the update divides by its
+** square root: the smallest steps of m and of sqrt(v) then lie equally far below their block's
+** largest, so what an element of m can be off by stays comparable with its own divisor.  A power of
+** two costs a float code no precision and makes scaling exact; no code is lost to rounding beyond
+** the top because 1.75 is the largest either code holds.  B = 255 says that the block held a
+** value that is not finite (or beyond 1.75 * 2^127): all of its moments read as NaN.
+**
+** Rounding is dithered: an average over a thousand steps (beta2 = 0.999) moves by less than half
+** a step of eight to the binade, so rounding to nearest would never let it move.  To the 20 bits
+** below the step a number of 16 random bits is added and the rest cut off: x rounds up with the
+** probability of its place between its neighbours, and its expectation stays.  The number is a hash
+** of the element's place in the flat and the step's count, so a run repeats bit for bit.  One
+** exception: a positive v never becomes 0 (the step would be divided by eps alone).
+*/
+constexpr int kQ8Block = 256;
+constexpr uint32_t kDitherGold = 0x9e3779b9u;	/* 2^32 / golden ratio */
+constexpr uint32_t kDitherMult = 0xb7e15163u;	/* 2^32 (e - 2), odd */
+
+__host__ __device__ __forceinline__ uint32_t dither_seed(uint32_t t)
+{
+	uint32_t s = (t * kDitherGold) ^ (t >> 7);
+
+	s *= kDitherMult;
+	return s ^ (s >> 16);
+}
+
+/* x = place * kDitherGold + seed -> 32 random bits: the low half for m, the high half for v. */
+__device__ __forceinline__ uint32_t dither_bits(uint32_t x)
+{
+	x ^= x >> 15;
+	x *= kDitherMult;
+	return x ^ (x >> 15);
+}
+
+/* The exponent byte for a block whose largest |x| has these bits (sign cleared). */
+__device__ __forceinline__ uint32_t q8_exponent(uint32_t abs_bits)
+{
+	const uint32_t b = (abs_bits + 0x1fffffu) >> 23;
+
+	return b < 255u ? b : 255u;
+}
+
+__device__ __forceinline__ int q8_top(uint32_t b)
+{
+	return (int)(b > 1u ? b : 1u) - 127;
+}
+
+/*
+** Codes.  A float whose exponent field is shifted into that of the code has the code in its bits
+** 20..27: E4M3 with bias 120 lower (2^-112-E scales 1.75 * 2^E to 1.75 * 2^-112), v's code with
+** 96 lower; below the smallest normal step the float is subnormal exactly where the code is, so
+** one integer addition and one shift round both ranges.
+*/
+__device__ __forceinline__ uint32_t q8_code_m(float m, int top, uint32_t dither20)
+{
+	const uint32_t u = __float_as_uint(m);
+	const uint32_t y = __float_as_uint(__builtin_ldexpf(__uint_as_float(u & 0x7fffffffu), -112 - top));
+
+	return ((y + dither20) >> 20) | ((u >> 24) & 0x80u);
+}
+
+__device__ __forceinline__ uint32_t q8_code_v(float v, int top, uint32_t dither20)
+{
+	const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+	const uint32_t y = __float_as_uint(__builtin_ldexpf(__uint_as_float(u), -96 - top));
+	const uint32_t c = (y + dither20) >> 20;
+	const uint32_t least = u < 1u ? u : 1u;
+
+	return c > least ? c : least;
+}
+
+/* Half a step, ties to even: what an import uses in the dither's place. */
+__device__ __forceinline__ uint32_t q8_nearest(float x, int shift)
+{
+	const uint32_t y = __float_as_uint(__builtin_ldexpf(__uint_as_float(__float_as_uint(x) & 0x7fffffffu), shift));
+
+	return 0x7ffffu + ((y >> 20) & 1u);
+}
+
+__device__ __forceinline__ float q8_value_m(uint32_t code, uint32_t b)
+{
+	const float x = __builtin_ldexpf(__builtin_amdgcn_cvt_f32_fp8((int)code, 0), q8_top(b) - 8);
+
+	return b == 255u ? __uint_as_float(0x7fc00000u) : x;
+}
+
+__device__ __forceinline__ float q8_value_v(uint32_t code, uint32_t b)
+{
+	const float x = __builtin_ldexpf(__uint_as_float(code << 20), q8_top(b) + 96);
+
+	return b == 255u ? __uint_as_float(0x7fc00000u) : x;
 }
 
 } /* namespace anni */

@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(HERE, "libanni_gpu_hip.so")
 BENCH_SO_PATH = os.path.join(HERE, "libanni_bench.so")
 
-F32, BF16, FP8_E4M3 = 0, 1, 2
+F32, BF16, FP8_E4M3, Q8 = 0, 1, 2, 3
 T_DECAY, T_TWIN, T_FP8TWIN = 1, 2, 4
 LAYOUT_AUTO, LAYOUT_COMPACT, LAYOUT_SPLIT = 0, 1, 2
 GPU_PREC_FP32, GPU_PREC_BF16 = 0, 1
@@ -116,6 +116,8 @@ _PROTOS = {
     "anni_adam_write_state": (C.c_int, [C.POINTER(Adam), C.c_int, C.c_int, C.c_int]),
     "anni_adam_read_state": (C.c_int, [C.POINTER(Adam), C.c_int, C.POINTER(C.c_int),
                                        C.POINTER(C.c_int)]),
+    "anni_adam_read_moments": (C.c_int, [C.POINTER(Adam), C.c_int64, C.c_int64, C.c_int, C.c_void_p,
+                                         C.c_void_p]),
     "anni_adam_enable_derived": (C.c_int, [C.POINTER(Adam), C.POINTER(Pack), C.c_int, C.c_int64]),
     "anni_gpu_device_info": (C.c_int, [C.c_char_p, C.c_size_t, C.POINTER(C.c_int)]),
     "anni_lr_set_schedule": (None, [C.c_int, C.c_int, C.c_char_p]),

@@ -11,7 +11,8 @@ import numpy as np
 
 from . import lib as _l
 
-_NP = {_l.F32: np.float32, _l.BF16: np.uint16, _l.FP8_E4M3: np.uint8}
+_NP = {_l.F32: np.float32, _l.BF16: np.uint16, _l.FP8_E4M3: np.uint8, _l.Q8: np.uint8}
+Q8_BLOCK = 256          # elements that share an exponent byte (moment_type Q8)
 
 
 def step_lr(base_lr, step, warmup=0, decay_steps=0, kind="none", sched_from=0):
@@ -203,6 +204,12 @@ class LmAdam:
         if self.L.anni_adam_import_mv(self.h, first, pairs.shape[0], pairs.ctypes.data) != 0:
             raise RuntimeError("anni_adam_import_mv failed")
 
+    def read_moments(self, m=None, v=None, first=0, count=None, out_type=_l.BF16):
+        """The moments of [first, first + count) as F32 or BF16 values at the device addresses m and v."""
+        count = self.n - first if count is None else count
+        if self.L.anni_adam_read_moments(self.h, first, count, out_type, m, v) != 0:
+            raise RuntimeError("anni_adam_read_moments refused or failed")
+
     def write_state(self, fd, epoch, step):
         """has_adam, epoch, step, t, n and the n pairs, as lm_save_checkpoint writes them."""
         if self.L.anni_adam_write_state(self.h, fd, epoch, step) != 0:
@@ -234,7 +241,14 @@ class LmAdam:
                 "m": (o.d_m, _NP[self.moment_type]), "v": (o.d_v, _NP[self.moment_type]),
                 "twin": (o.d_param_bf16, np.uint16), "gscale": (o.d_gscale, np.float32),
                 "fp8twin": (o.d_param_fp8, np.uint8), "wscale": (o.d_wscale, np.float32),
-                "pack": (o.d_pack_bf16, np.uint16)}[which]
+                "pack": (o.d_pack_bf16, np.uint16),
+                "m_exp": ((o.d_m or 0) + self.blocks * Q8_BLOCK, np.uint8),
+                "v_exp": ((o.d_v or 0) + self.blocks * Q8_BLOCK, np.uint8)}[which]
+
+    @property
+    def blocks(self):
+        """Blocks of 8-bit moments in the flat."""
+        return (self.n + Q8_BLOCK - 1) // Q8_BLOCK
 
     def upload(self, which, arr, offset=0):
         ptr, dt = self._flat(which)
@@ -255,7 +269,8 @@ class LmAdam:
         ptr, dt = self._flat(which)
         if count is None:
             count = (self.o.n_tensors if which in ("gscale", "wscale")
-                     else self.pack_elems if which == "pack" else self.n)
+                     else self.pack_elems if which == "pack"
+                     else self.blocks if which in ("m_exp", "v_exp") else self.n)
         out = np.empty(count, dtype=dt)
         if self.L.gpu_memcpy_d2h(out.ctypes.data, ptr + offset * out.itemsize, out.nbytes) != 0:
             raise RuntimeError("download(%s) failed" % which)

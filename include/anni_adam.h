@@ -36,6 +36,24 @@ extern "C" {
 #define ANNI_F32	0
 #define ANNI_BF16	1	/* upper 16 bits of an IEEE float */
 #define ANNI_FP8_E4M3	2	/* OCP E4M3: bias 7, max 448, S.1111.111 = NaN, no infinities */
+/*
+** Moments in 8 bits (moment_type only).  The flat is cut into blocks of 256 elements, counted from
+** its start whatever the tensors; a moment is an 8-bit float times a power of two of its block.
+**   exponent byte B, E = max(B, 1) - 127, the least E with max |x| <= 1.75 * 2^E
+**   m  E4M3 code (as ANNI_FP8_E4M3) * 2^(E - 8)
+**   v  unsigned code, five exponent and three fraction bits: field f > 0: (1 + r / 8) * 2^(E + f - 31),
+**      field 0: r * 2^(E - 33)
+** d_m and d_v hold ceil(n / 256) * 256 code bytes, then ceil(n / 256) exponent bytes: 2.008 bytes
+** per parameter for both, against 8 with ANNI_F32.  The step computes with the decoded values in
+** double like every other mode, uses the new moments unrounded, and then rounds them to the
+** formats with a dither: up with the probability of the place between the two neighbours, by a
+** hash of the element's index and t, so that averages as slow as beta2 = 0.999 still move (to
+** nearest they would not: a step's change is less than half a code) and runs repeat bit for bit.
+** A positive v is stored as at least the smallest code.  A block that holds a value that is not
+** finite reads as NaN as a whole (B = 255); skip_nonfinite keeps such gradients out.  Values below
+** the smallest float (a block of v whose largest is under 2^-116) lose bits when they are read.
+*/
+#define ANNI_Q8		3
 
 /*
 ** Arena layouts.  MI355X's device memory behaves as three sections of 96 GiB, and a kernel
@@ -67,7 +85,7 @@ typedef struct anni_tensor {
 
 typedef struct anni_adam_config {
 	int	grad_type;	/* ANNI_F32 / ANNI_BF16 / ANNI_FP8_E4M3 */
-	int	moment_type;	/* ANNI_F32 / ANNI_BF16 (computed in double, rounded f32 then bf16 on store) */
+	int	moment_type;	/* ANNI_F32 / ANNI_BF16 (computed in double, rounded f32 then bf16 on store) / ANNI_Q8 */
 	int	twins;		/* 1: allocate the bf16 twin flat */
 	int	skip_nonfinite;	/* 1: a non-finite gradient norm skips the update (lm_adam.c:474-483) */
 	int	grad_slots;	/* gradient flats the arena allocates (slot 0 starts bound); 0: bind one with anni_adam_bind_grad */
@@ -240,7 +258,11 @@ int	anni_adam_sync_stats(anni_adam *opt);
 ** The optimizer block of the reference's checkpoint (lang/lm_serialize.c:263-331,526-587):
 ** five int32 {1, epoch, step, t, n} followed by n (m, v) float pairs in slot order, written
 ** from / read into the arena through an interleave kernel and page-locked staging in chunks
-** of 2^21 slots.  bf16 moments widen exactly on export and round to nearest even on import.
+** of 2^21 slots.  bf16 moments widen exactly on export and round to nearest even on import;
+** so do 8-bit ones, and exporting and importing a whole state gives its values back.  An import of a range that
+** begins or ends inside a block of 8-bit moments encodes the block's other slots anew under the
+** block's new exponent (they keep their values unless it grew past their smallest bits); a
+** negative v becomes 0 there.
 ** export / import move the pairs of slots [first, first+count) to / from host memory;
 ** write / read move the whole block through a file descriptor (read restores t).
 */
@@ -248,6 +270,16 @@ int	anni_adam_export_mv(anni_adam *opt, int64_t first, int64_t count, float *pai
 int	anni_adam_import_mv(anni_adam *opt, int64_t first, int64_t count, const float *pairs);
 int	anni_adam_write_state(anni_adam *opt, int fd, int epoch, int step);
 int	anni_adam_read_state(anni_adam *opt, int fd, int *epoch, int *step);
+
+/*
+** The moments of elements [first, first + count) as values on the device: d_m[k] and d_v[k] receive
+** those of element first + k as ANNI_F32 or ANNI_BF16 (`type`; round to nearest even), whatever the
+** arena stores; either may be NULL, both are aligned to an element.  For looking at a state or
+** carrying it into an arena of another moment_type without the trip through the host that
+** export_mv makes.  Asynchronous on the compute stream unless the moments are offloaded.
+*/
+int	anni_adam_read_moments(anni_adam *opt, int64_t first, int64_t count, int type, void *d_m,
+		void *d_v);
 
 /* lm_train_step_lr and its setters (lang/lm_train.c:98-124,398-411); kind "none" / "linear" / "cosine". */
 void	anni_lr_set_schedule(int warmup_steps, int decay_steps, const char *kind);
