@@ -1,0 +1,1015 @@
+/*
+** Softmax cross entropy of the language model's head over the whole vocabulary, with its gradients,
+** without the logits in memory (include/anni_adam.h, "the head's loss").
+**
+**   logits l[i][v] = sum_d x[i][d] w[d][v] + b[v]
+**   nll[i] = log sum_v exp(l[i][v]) - l[i][target_i]
+**   delta[i][v] = scale (exp(l[i][v] - lse_i) - [v = target_i])
+**   dx = delta w^T,  dw += x^T delta,  db += sum_i delta[i]
+**
+** Four products, two of them the same: the first pass over the vocabulary keeps a running maximum
+** and sum per token and throws the logits away; the second forms them again, a piece of the
+** vocabulary at a time, turns them into delta (bf16, in the work area) and the other two products
+** read it.  Recomputing costs a third more operations than the 6 rows d vocab that cannot be
+** avoided; keeping the logits would cost 4 rows vocab bytes.  With float gradients delta is kept as
+** the sum of two bf16 numbers (16 bits of fraction, an error of 2^-17 against 2^-9), and the two
+** products that read it run over both.
+**
+** All products are the one kernel below on bf16 operands with float sums: a workgroup of eight
+** wavefronts owns a tile of the result, walks the contracted axis in steps of 64 with the next
+** step's operands on the way into registers, and feeds 32 x 32 x 16 matrix instructions from LDS.
+** An operand lies in memory either with the contracted axis contiguous, or with its rows contiguous;
+** the second kind is turned by the transposing LDS read, so nothing is transposed in memory.
+*/
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <string.h>
+#include "adam_kernels.h"
+#include "anni_adam.h"
+#include "backend_state.h"
+
+namespace anni {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+/* sixteen bytes at any element: rows of an odd vocabulary are not aligned (the hardware does not mind) */
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+constexpr int kHeadThreads = 512;	/* eight wavefronts, two to a SIMD */
+constexpr int kStep = 64;		/* of the contracted axis per trip */
+constexpr int kSide = 256;		/* of a result tile along the vocabulary or the model's width */
+
+#define ANNI_LDS __attribute__((address_space(3)))
+
+/*
+** One operand of a product: element (r, k), 0 <= r < ROWS of the tile, k of a step.  BY_ROW: the
+** rows are contiguous (element (r, k) at k ld + r), else the contracted axis (r ld + k).  CHECK: the
+** array ends inside tiles; loads never leave it: what lies beyond along the contiguous axis reads as
+** 0, beyond along the other one the last valid line again (its product is with zeros, or not kept).
+** LDS image: 16-byte chunks, those of a line rotated by an exclusive or so that the lanes of a
+** fragment read spread over all banks.
+*/
+struct Source {
+	const uint16_t	*part[2];	/* second: the low halves, same shape */
+	uint32_t	ld;
+	int64_t		rows;		/* valid rows from row 0 */
+	int64_t		depth;		/* valid length of the contracted axis */
+};
+
+template <bool BY_ROW, bool CHECK, int ROWS>
+struct Operand {
+	static constexpr int kChunks = ROWS * kStep / 8 / kHeadThreads;
+	static constexpr int kBytes = ROWS * kStep * 2;
+	u32x4	hold[kChunks];
+
+	/* step `s` of `steps` per part */
+	__device__ __forceinline__ void fetch(const Source &src, int64_t row0, int s, int steps, int tid)
+	{
+		const int part = s >= steps ? 1 : 0;
+		const int64_t k0 = (int64_t)(s - part * steps) * kStep;
+		const uint16_t *base = src.part[part] + (BY_ROW ? k0 * src.ld + row0 : row0 * src.ld + k0);
+		const int64_t rows_left = src.rows - row0;
+		const int64_t depth_left = src.depth - k0;
+		const bool inside = !CHECK || (rows_left >= ROWS && depth_left >= kStep);
+
+#pragma unroll
+		for (int i = 0; i < kChunks; i++) {
+			const int c = tid + i * kHeadThreads;
+			const int line = BY_ROW ? c / (ROWS / 8) : c / (kStep / 8);
+			const int col = (BY_ROW ? c % (ROWS / 8) : c % (kStep / 8)) * 8;
+
+			if (inside) {
+				hold[i] = *(const u32x4_any *)(base + ((uint32_t)line * src.ld + (uint32_t)col));
+			} else {
+				const int64_t lines = BY_ROW ? depth_left : rows_left;
+				const int64_t cols = BY_ROW ? rows_left : depth_left;
+				const uint16_t *p = base + (uint32_t)(line < lines ? line : (int)lines - 1) * src.ld;
+				u32x4 w = {0u, 0u, 0u, 0u};
+
+				if (col + 8 <= cols) {
+					w = *(const u32x4_any *)(p + col);
+				} else {
+					/* from the last element down, each pushing the others up */
+#pragma unroll 1
+					for (int j = 7; j >= 0; j--) {
+						const uint32_t e = col + j < cols ? p[col + j] : 0u;
+
+						w.w = (w.w << 16) | (w.z >> 16);
+						w.z = (w.z << 16) | (w.y >> 16);
+						w.y = (w.y << 16) | (w.x >> 16);
+						w.x = (w.x << 16) | e;
+					}
+				}
+				hold[i] = w;
+			}
+		}
+	}
+
+	static __device__ __forceinline__ uint32_t place(int line, int chunk)
+	{
+		if (BY_ROW)
+			return (uint32_t)line * (ROWS * 2) + (uint32_t)((chunk ^ ((line & 3) << 2)) * 16);
+		return (uint32_t)line * (kStep * 2) + (uint32_t)((chunk ^ (line & 7)) * 16);
+	}
+
+	__device__ __forceinline__ void put(char *lds, int tid) const
+	{
+#pragma unroll
+		for (int i = 0; i < kChunks; i++) {
+			const int c = tid + i * kHeadThreads;
+			const int line = BY_ROW ? c / (ROWS / 8) : c / (kStep / 8);
+			const int chunk = BY_ROW ? c % (ROWS / 8) : c % (kStep / 8);
+
+			*(u32x4 *)(lds + place(line, chunk)) = hold[i];
+		}
+	}
+
+	/* Fragment of a 32 x 32 x 16 product: lane l holds row r0 + l % 32, places 16 sub + 8 (l / 32) .. + 7. */
+	static __device__ __forceinline__ bf16x8 fragment(const char *lds, int r0, int sub, int lane)
+	{
+		if constexpr (BY_ROW) {
+			/* each 16 lanes read four lines of 16 rows and get them turned: a lane one row of four lines */
+			const int line = sub * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
+			const int row = r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+			const uint32_t half = (uint32_t)(row & 4) * 2;
+			union { i16x4 h[2]; bf16x8 f; } u;
+
+			u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ANNI_LDS i16x4 *)(lds + place(line, row >> 3) + half));
+			u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ANNI_LDS i16x4 *)(lds + place(line + 4, row >> 3) + half));
+			return u.f;
+		} else {
+			return *(const bf16x8 *)(lds + place(r0 + (lane & 31), sub * 2 + (lane >> 5)));
+		}
+	}
+};
+
+/* acc += A B^T over the steps [from, to): acc[i][j] is the 32 x 32 block (i, j) of the wavefront's part. */
+template <class A, class B, int MB, int NB>
+__device__ __forceinline__ void product(f32x16 (&acc)[MB][NB], const Source &sa, const Source &sb, int64_t row_a,
+	int64_t row_b, int from, int to, int steps, char *lds, int ra, int rb, int tid)
+{
+	A a;
+	B b;
+	const int lane = tid & 63;
+	constexpr int kBuffer = A::kBytes + B::kBytes;
+	int at = 0;
+
+	if (from >= to)
+		return;		/* an empty slice; the same in every lane of the workgroup */
+	a.fetch(sa, row_a, from, steps, tid);
+	b.fetch(sb, row_b, from, steps, tid);
+	a.put(lds, tid);
+	b.put(lds + A::kBytes, tid);
+	__syncthreads();
+	for (int s = from; s < to; s++) {
+		const char *la = lds + at * kBuffer;
+		const char *lb = la + A::kBytes;
+
+		if (s + 1 < to) {
+			a.fetch(sa, row_a, s + 1, steps, tid);
+			b.fetch(sb, row_b, s + 1, steps, tid);
+		}
+#pragma unroll
+		for (int sub = 0; sub < kStep / 16; sub++) {
+			bf16x8 fa[MB], fb[NB];
+
+#pragma unroll
+			for (int i = 0; i < MB; i++)
+				fa[i] = A::fragment(la, ra + i * 32, sub, lane);
+#pragma unroll
+			for (int j = 0; j < NB; j++)
+				fb[j] = B::fragment(lb, rb + j * 32, sub, lane);
+#pragma unroll
+			for (int i = 0; i < MB; i++)
+#pragma unroll
+				for (int j = 0; j < NB; j++)
+					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+		}
+		if (s + 1 < to) {
+			/* the other buffer: its last readers passed the barrier at the end of the step before */
+			at ^= 1;
+			a.put(lds + at * kBuffer, tid);
+			b.put(lds + at * kBuffer + A::kBytes, tid);
+		}
+		__syncthreads();
+	}
+}
+
+/* Row of register r of a 32 x 32 block in lane l; the column is l % 32. */
+__device__ __forceinline__ int block_row(int r, int lane)
+{
+	return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+}
+
+/*
+** Which tile a workgroup takes.  Consecutive workgroups go to the eight dies in turn, so die x gets
+** the x-th eighth of the list, and the list runs over bands of eight tiles of the short axis: what a
+** die works on at one time shares operands in its level-two cache.
+*/
+__device__ __forceinline__ bool tile_of(int64_t id, int64_t tiles_a, int64_t tiles_b, int64_t *ta, int64_t *tb)
+{
+	const int64_t n = tiles_a * tiles_b;
+	const int64_t per = (n + 7) / 8;
+	const int64_t at = (id & 7) * per + (id >> 3);
+	const int64_t band = 8 * tiles_a;
+
+	if ((id >> 3) >= per || at >= n)
+		return false;
+	const int64_t g = at / band;
+	const int64_t in = at - g * band;
+	const int64_t wide = tiles_b - g * 8 < 8 ? tiles_b - g * 8 : 8;
+
+	*ta = in / wide;
+	*tb = g * 8 + in % wide;
+	return true;
+}
+
+/* ---- rows: a clean copy of x and of the targets --------------------------------------------- */
+
+struct RowArgs {
+	const uint16_t	*x;
+	int64_t		ld_x;
+	const int32_t	*target;
+	int64_t		rows, rows_pad;
+	int		d, d_pad, vocab;
+	int64_t		vocab_pad;
+	const float	*bias;		/* may be NULL */
+	uint16_t	*xs;
+	int32_t		*ts;
+	float		*bs;
+};
+
+/*
+** xs[rows_pad][d_pad] = x, with zeros for rows without a target (whatever x holds there) and beyond
+** rows and d; ts = target, -1 for rows without one; bs = bias, -inf beyond the vocabulary (which has
+** probability 0 there, and so no delta).  The products then need no masks.
+*/
+__global__ __launch_bounds__(kThreads) void head_rows_kernel(RowArgs a)
+{
+	const int64_t per = a.d_pad / 8;
+	const int64_t n = a.rows_pad * per;
+
+	for (int64_t q = (int64_t)blockIdx.x * kThreads + threadIdx.x; q < n; q += (int64_t)gridDim.x * kThreads) {
+		const int64_t r = q / per;
+		const int c = (int)(q - r * per) * 8;
+		const int32_t t = r < a.rows ? a.target[r] : -1;
+		const bool live = t >= 0 && t < a.vocab;
+		u32x4 w = {0u, 0u, 0u, 0u};
+
+		if (live && c + 8 <= a.d) {
+			w = *(const u32x4_any *)(a.x + r * a.ld_x + c);
+		} else if (live) {
+			uint32_t e[4] = {0u, 0u, 0u, 0u};
+
+			for (int j = 0; j < 8; j++)
+				if (c + j < a.d)
+					e[j / 2] |= (uint32_t)a.x[r * a.ld_x + c + j] << (16 * (j & 1));
+			w = u32x4{e[0], e[1], e[2], e[3]};
+		}
+		*(u32x4 *)(a.xs + r * a.d_pad + c) = w;
+		if (c == 0)
+			a.ts[r] = live ? t : -1;
+	}
+	for (int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x; v < a.vocab_pad;
+	    v += (int64_t)gridDim.x * kThreads)
+		a.bs[v] = v >= a.vocab ? -INFINITY : a.bias ? a.bias[v] : 0.0f;
+}
+
+/* ---- logits, by tile: their softmax's running statistics, or delta ----------------------------- */
+
+struct LogitArgs {
+	Source		w;		/* by row: w[d][vocab] */
+	Source		x;		/* xs */
+	const float	*bias;		/* bs */
+	const int32_t	*target;	/* ts */
+	int		steps;
+	int64_t		tiles_v, tiles_t;
+	int64_t		rows_pad;
+	/* statistics */
+	f32x2		*part;		/* [tiles_v][rows_pad]: maximum, sum of exp(l - maximum) */
+	float		*target_logit;
+	/* delta */
+	const float	*lse;
+	float		scale;
+	int64_t		v0;		/* first vocabulary place of this piece */
+	uint16_t	*delta;		/* [rows_pad][ld_delta], low halves behind the high ones */
+	uint16_t	*delta_low;
+	int64_t		ld_delta;
+};
+
+enum { kStats = 0, kDelta = 1, kDeltaPair = 2 };
+
+template <int TT> struct LogitWaves { static constexpr int m = TT == 256 ? 2 : TT == 128 ? 4 : 8, n = 8 / m; };
+
+template <int TT, int MODE>
+__global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
+{
+	typedef Operand<true, true, kSide> W;
+	typedef Operand<false, false, TT> X;
+	constexpr int WM = LogitWaves<TT>::m, WN = LogitWaves<TT>::n;
+	constexpr int MB = kSide / WM / 32, NB = TT / WN / 32;
+	__shared__ __align__(16) char lds[2 * (W::kBytes + X::kBytes)];
+	const int tid = threadIdx.x;
+	const int lane = tid & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int wm = wave / WN, wn = wave % WN;
+	int64_t tv, tt;
+	f32x16 acc[MB][NB];
+
+	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_t, &tv, &tt))
+		return;
+	const int64_t v_tile = a.v0 + tv * kSide;
+	const int64_t t_tile = tt * TT;
+	const int64_t v_base = v_tile + wm * (MB * 32);
+
+#pragma unroll
+	for (int i = 0; i < MB; i++)
+#pragma unroll
+		for (int j = 0; j < NB; j++)
+			acc[i][j] = f32x16{};
+	product<W, X, MB, NB>(acc, a.w, a.x, v_tile, t_tile, 0, a.steps, a.steps, lds, wm * (MB * 32), wn * (NB * 32),
+	    tid);
+#pragma unroll
+	for (int i = 0; i < MB; i++)
+#pragma unroll
+		for (int q = 0; q < 4; q++) {
+			const f32x4 b = *(const f32x4 *)(a.bias + v_base + i * 32 + block_row(4 * q, lane));
+
+#pragma unroll
+			for (int j = 0; j < NB; j++)
+#pragma unroll
+				for (int k = 0; k < 4; k++)
+					acc[i][j][4 * q + k] += b[k];
+			if ((q & 1) == 1)
+				__builtin_amdgcn_sched_barrier(0);	/* all loads ahead of all sums take registers that there are not */
+		}
+	if constexpr (MODE == kStats) {
+		f32x2 *red = (f32x2 *)lds;	/* [WM][TT]; product() ended with a barrier */
+
+#pragma unroll
+		for (int j = 0; j < NB; j++) {
+			const int t = wn * (NB * 32) + j * 32 + (lane & 31);
+			const int64_t want = (int64_t)a.target[t_tile + t] - v_base;
+			float top = -INFINITY, sum = 0.0f, hit = 0.0f;
+
+#pragma unroll
+			for (int i = 0; i < MB; i++)
+#pragma unroll
+				for (int r = 0; r < 16; r++) {
+					top = fmaxf(top, acc[i][j][r]);
+					if (want == i * 32 + block_row(r, lane))
+						hit = acc[i][j][r];
+				}
+			top = fmaxf(top, __shfl_xor(top, 32, 64));
+			/* nothing but -inf: every exponential is 0 against any finite maximum */
+			const float ref = top == -INFINITY ? 0.0f : top;
+
+#pragma unroll
+			for (int i = 0; i < MB; i++)
+#pragma unroll
+				for (int r = 0; r < 16; r++)
+					sum += __expf(acc[i][j][r] - ref);
+			sum += __shfl_xor(sum, 32, 64);
+			if (lane < 32)
+				red[wm * TT + t] = f32x2{top, sum};
+			if (want >= 0 && want < MB * 32 && (int)((want >> 2) & 1) == (lane >> 5))
+				a.target_logit[t_tile + t] = hit;
+		}
+		__syncthreads();
+		for (int t = tid; t < TT; t += kHeadThreads) {
+			float top = -INFINITY, sum = 0.0f;
+
+#pragma unroll
+			for (int k = 0; k < WM; k++)
+				top = fmaxf(top, red[k * TT + t].x);
+			const float ref = top == -INFINITY ? 0.0f : top;
+
+#pragma unroll
+			for (int k = 0; k < WM; k++)
+				sum += red[k * TT + t].y * __expf(red[k * TT + t].x - ref);
+			a.part[tv * a.rows_pad + t_tile + t] = f32x2{top, sum};
+		}
+	} else {
+#pragma unroll
+		for (int j = 0; j < NB; j++) {
+			const int64_t t = t_tile + wn * (NB * 32) + j * 32 + (lane & 31);
+			const int64_t want = (int64_t)a.target[t] - v_base;
+			const bool live = a.target[t] >= 0;
+			const float lse = a.lse[t];
+
+#pragma unroll
+			for (int i = 0; i < MB; i++)
+#pragma unroll
+				for (int q = 0; q < 4; q++) {
+					const int row = i * 32 + block_row(4 * q, lane);
+					const int64_t at = t * a.ld_delta + (v_base - a.v0) + row;
+					float e[4], low[4];
+					u32x2 w;
+
+#pragma unroll
+					for (int k = 0; k < 4; k++) {
+						float p = __expf(acc[i][j][4 * q + k] - lse);
+
+						if (want == row + k)
+							p -= 1.0f;
+						e[k] = live ? p * a.scale : 0.0f;
+					}
+					w.x = bf16_rne2(e[0], e[1]);
+					w.y = bf16_rne2(e[2], e[3]);
+					*(u32x2 *)(a.delta + at) = w;
+					if constexpr (MODE == kDeltaPair) {
+						/* what the rounding left over, rounded itself */
+						low[0] = e[0] - __uint_as_float(w.x << 16);
+						low[1] = e[1] - __uint_as_float(w.x & 0xffff0000u);
+						low[2] = e[2] - __uint_as_float(w.y << 16);
+						low[3] = e[3] - __uint_as_float(w.y & 0xffff0000u);
+						w.x = bf16_rne2(low[0], low[1]);
+						w.y = bf16_rne2(low[2], low[3]);
+						*(u32x2 *)(a.delta_low + at) = w;
+					}
+				}
+		}
+	}
+}
+
+/* ---- the statistics of all tiles -> lse and nll ------------------------------------------------ */
+
+struct FinishArgs {
+	const f32x2	*part;
+	const float	*target_logit;
+	const int32_t	*target;
+	int64_t		tiles_v, rows, rows_pad;
+	float		*lse;
+	float		*nll;
+};
+
+/* 64 tokens to a workgroup, its sixteen wavefronts share the tiles; folded in a fixed order. */
+constexpr int kFinishWaves = 16;
+
+__global__ __launch_bounds__(kFinishWaves * 64) void head_finish_kernel(FinishArgs a)
+{
+	__shared__ f32x2 red[kFinishWaves][64];
+	const int lane = threadIdx.x & 63;
+	const int wave = threadIdx.x >> 6;
+	const int64_t t = (int64_t)blockIdx.x * 64 + lane;
+	float top = -INFINITY, sum = 0.0f;
+
+	for (int64_t k = wave; k < a.tiles_v; k += kFinishWaves) {
+		const f32x2 p = a.part[k * a.rows_pad + t];
+		const float m = fmaxf(top, p.x);
+		const float ref = m == -INFINITY ? 0.0f : m;
+
+		sum = sum * __expf(top - ref) + p.y * __expf(p.x - ref);
+		top = m;
+	}
+	red[wave][lane] = f32x2{top, sum};
+	__syncthreads();
+	if (wave != 0)
+		return;
+	for (int k = 1; k < kFinishWaves; k++) {
+		const f32x2 p = red[k][lane];
+		const float m = fmaxf(top, p.x);
+		const float ref = m == -INFINITY ? 0.0f : m;
+
+		sum = sum * __expf(top - ref) + p.y * __expf(p.x - ref);
+		top = m;
+	}
+	const bool live = a.target[t] >= 0;
+	const float log_sum = logf(sum);
+
+	if (a.lse)
+		a.lse[t] = top + log_sum;
+	if (t < a.rows)
+		a.nll[t] = live ? (top - a.target_logit[t]) + log_sum : 0.0f;
+}
+
+/* ---- dx ---------------------------------------------------------------------------------------- */
+
+struct DxArgs {
+	Source		delta;
+	Source		w;
+	int		steps, parts, splits;
+	int64_t		tiles_t, tiles_d;
+	float		*slot;		/* [splits][rows_pad][d_pad] */
+	int64_t		rows_pad;
+	int		d_pad;
+	int		add;		/* later pieces of the vocabulary add to the slots */
+};
+
+/* One slice of the contracted axis (the vocabulary) per blockIdx.y, each with a slot of its own. */
+template <int TT>
+__global__ __launch_bounds__(kHeadThreads) void head_dx_kernel(DxArgs a)
+{
+	typedef Operand<false, false, TT> D;
+	typedef Operand<false, true, kSide> W;
+	constexpr int WM = 2, WN = 4;
+	constexpr int MB = TT / WM / 32, NB = kSide / WN / 32;
+	__shared__ __align__(16) char lds[2 * (D::kBytes + W::kBytes)];
+	const int tid = threadIdx.x;
+	const int lane = tid & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int wm = wave / WN, wn = wave % WN;
+	const int total = a.steps * a.parts;
+	const int from = (int)((int64_t)total * blockIdx.y / a.splits);
+	const int to = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
+	int64_t tt, td;
+	f32x16 acc[MB][NB];
+
+	if (!tile_of(blockIdx.x, a.tiles_t, a.tiles_d, &tt, &td))
+		return;
+#pragma unroll
+	for (int i = 0; i < MB; i++)
+#pragma unroll
+		for (int j = 0; j < NB; j++)
+			acc[i][j] = f32x16{};
+	product<D, W, MB, NB>(acc, a.delta, a.w, tt * TT, td * kSide, from, to, a.steps, lds, wm * (MB * 32),
+	    wn * (NB * 32), tid);
+#pragma unroll
+	for (int i = 0; i < MB; i++)
+#pragma unroll
+		for (int j = 0; j < NB; j++)
+#pragma unroll
+			for (int r = 0; r < 16; r++) {
+				const int64_t t = tt * TT + wm * (MB * 32) + i * 32 + block_row(r, lane);
+				const int64_t c = td * kSide + wn * (NB * 32) + j * 32 + (lane & 31);
+				float *p = a.slot + ((int64_t)blockIdx.y * a.rows_pad + t) * a.d_pad + c;
+
+				*p = a.add ? *p + acc[i][j][r] : acc[i][j][r];
+			}
+}
+
+struct DxSumArgs {
+	const float	*slot;
+	int		splits;
+	int64_t		rows, rows_pad;
+	int		d, d_pad;
+	void		*dx;
+	int64_t		ld_dx;
+};
+
+/* dx = the slots' sum in order, in the caller's type. */
+template <int GT>
+__global__ __launch_bounds__(kThreads) void head_dx_sum_kernel(DxSumArgs a)
+{
+	const int64_t per = a.d_pad / 4;
+	const int64_t n = a.rows * per;
+
+	for (int64_t q = (int64_t)blockIdx.x * kThreads + threadIdx.x; q < n; q += (int64_t)gridDim.x * kThreads) {
+		const int64_t r = q / per;
+		const int c = (int)(q - r * per) * 4;
+		f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+
+		if (c >= a.d)
+			continue;
+		for (int k = 0; k < a.splits; k++)
+			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_pad + c);
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+			if (c + j < a.d) {
+				if constexpr (GT == kF32)
+					((float *)a.dx)[r * a.ld_dx + c + j] = s[j];
+				else
+					((uint16_t *)a.dx)[r * a.ld_dx + c + j] = (uint16_t)bf16_rne(s[j]);
+			}
+	}
+}
+
+/* ---- dw and db --------------------------------------------------------------------------------- */
+
+struct DwArgs {
+	Source		x;
+	Source		delta;
+	int		steps, parts;
+	int64_t		tiles_d, tiles_v;
+	int		d, vocab;
+	int64_t		v0;
+	void		*dw;		/* [d][vocab] */
+	void		*db;		/* [vocab] or NULL */
+};
+
+template <int GT>
+__device__ __forceinline__ void add_to(void *base, int64_t i, float x)
+{
+	if constexpr (GT == kF32)
+		((float *)base)[i] += x;
+	else
+		((uint16_t *)base)[i] = (uint16_t)bf16_rne(bf16_widen(((uint16_t *)base)[i]) + x);
+}
+
+template <int GT>
+__global__ __launch_bounds__(kHeadThreads) void head_dw_kernel(DwArgs a)
+{
+	typedef Operand<true, false, kSide> X;
+	typedef Operand<true, false, kSide> D;
+	constexpr int WM = 2, WN = 4;
+	constexpr int MB = kSide / WM / 32, NB = kSide / WN / 32;
+	__shared__ __align__(16) char lds[2 * (X::kBytes + D::kBytes)];
+	const int tid = threadIdx.x;
+	const int lane = tid & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int wm = wave / WN, wn = wave % WN;
+	int64_t td, tv;
+	f32x16 acc[MB][NB];
+
+	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_d, &tv, &td))
+		return;
+#pragma unroll
+	for (int i = 0; i < MB; i++)
+#pragma unroll
+		for (int j = 0; j < NB; j++)
+			acc[i][j] = f32x16{};
+	product<X, D, MB, NB>(acc, a.x, a.delta, td * kSide, tv * kSide, 0, a.steps * a.parts, a.steps, lds,
+	    wm * (MB * 32), wn * (NB * 32), tid);
+#pragma unroll
+	for (int j = 0; j < NB; j++) {
+		const int64_t v = a.v0 + tv * kSide + wn * (NB * 32) + j * 32 + (lane & 31);
+
+		if (v >= a.vocab)
+			continue;
+#pragma unroll
+		for (int i = 0; i < MB; i++)
+#pragma unroll
+			for (int r = 0; r < 16; r++) {
+				const int64_t c = td * kSide + wm * (MB * 32) + i * 32 + block_row(r, lane);
+
+				if (c < a.d)
+					add_to<GT>(a.dw, c * a.vocab + v, acc[i][j][r]);
+			}
+	}
+}
+
+struct DbArgs {
+	const uint16_t	*delta[2];
+	int		parts;
+	int64_t		ld, rows_pad;
+	int64_t		v0;
+	int		count;		/* columns of this piece */
+	void		*db;
+};
+
+/* db += column sums of delta: 64 columns to a workgroup, rows shared by its wavefronts, fixed order. */
+template <int GT>
+__global__ __launch_bounds__(kHeadThreads) void head_db_kernel(DbArgs a)
+{
+	__shared__ float red[8][64];
+	const int lane = threadIdx.x & 63;
+	const int wave = threadIdx.x >> 6;
+	const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+	float s = 0.0f;
+
+	for (int p = 0; p < a.parts; p++)
+		for (int64_t r = wave; r < a.rows_pad; r += 8)
+			s += bf16_widen(a.delta[p][r * a.ld + c]);
+	red[wave][lane] = s;
+	__syncthreads();
+	if (wave == 0 && c < a.count) {
+		for (int k = 1; k < 8; k++)
+			s += red[k][lane];
+		add_to<GT>(a.db, a.v0 + c, s);
+	}
+}
+
+/* ---- plan -------------------------------------------------------------------------------------- */
+
+struct HeadPlan {
+	int	tile_t;		/* tokens per tile */
+	int64_t	rows_pad;
+	int	d_pad;
+	int64_t	tiles_v;	/* of the whole vocabulary */
+	int64_t	piece;		/* vocabulary places per piece of delta, a multiple of kSide */
+	int	parts;		/* bf16 numbers per element of delta */
+	int	splits;		/* slices of the vocabulary in dx */
+	size_t	off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_slot;
+	size_t	bytes;
+};
+
+static size_t up(size_t x, size_t a)
+{
+	return (x + a - 1) / a * a;
+}
+
+static const int64_t kHeadMaxRows = (int64_t)1 << 22;
+static const int kHeadMaxD = 1 << 16;
+static const int kHeadMaxVocab = 1 << 22;
+
+/* grad_type: -1 = the loss alone. */
+static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p)
+{
+	const size_t delta_most = (size_t)512 << 20;
+	size_t at = 0;
+
+	if (rows <= 0 || rows > kHeadMaxRows || d <= 0 || d > kHeadMaxD || vocab <= 0 || vocab > kHeadMaxVocab
+	    || (grad_type != -1 && grad_type != ANNI_F32 && grad_type != ANNI_BF16))
+		return false;
+	memset(p, 0, sizeof(*p));
+	p->tile_t = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+	p->rows_pad = (int64_t)up((size_t)rows, (size_t)p->tile_t);
+	p->d_pad = (int)up((size_t)d, kSide);
+	p->tiles_v = (vocab + kSide - 1) / kSide;
+	p->parts = grad_type == ANNI_F32 ? 2 : 1;
+	p->off_xs = at;
+	at = up(at + (size_t)p->rows_pad * p->d_pad * 2, 256);
+	p->off_ts = at;
+	at = up(at + (size_t)p->rows_pad * 4, 256);
+	p->off_bs = at;
+	at = up(at + (size_t)p->tiles_v * kSide * 4, 256);
+	p->off_part = at;
+	at = up(at + (size_t)p->tiles_v * p->rows_pad * 8, 256);
+	p->off_hit = at;
+	at = up(at + (size_t)p->rows_pad * 4, 256);
+	p->off_lse = at;
+	at = up(at + (size_t)p->rows_pad * 4, 256);
+	if (grad_type != -1) {
+		const int64_t whole = p->tiles_v * kSide;
+		const int64_t fit = (int64_t)(delta_most / ((size_t)p->rows_pad * 2 * p->parts)) / kSide * kSide;
+		const int64_t tiles = p->rows_pad / p->tile_t * (p->d_pad / kSide);
+		int64_t steps;
+
+		p->piece = whole <= fit ? whole : fit < kSide ? kSide : fit;
+		steps = p->piece / kStep * p->parts;
+		p->splits = 1;
+		while (tiles * p->splits < 512 && steps / (p->splits * 2) >= 8)
+			p->splits *= 2;
+		p->off_delta = at;
+		at = up(at + (size_t)p->rows_pad * p->piece * 2 * p->parts, 256);
+		p->off_slot = at;
+		at = up(at + (size_t)p->splits * p->rows_pad * p->d_pad * 4, 256);
+	}
+	p->bytes = at;
+	return true;
+}
+
+static int rows_grid(int64_t items)
+{
+	const int64_t g = (items + kThreads - 1) / kThreads;
+
+	return (int)(g > 8192 ? 8192 : g < 1 ? 1 : g);
+}
+
+template <int MODE>
+static void logits_launch(hipStream_t st, int tile_t, const LogitArgs &a)
+{
+	const dim3 grid((unsigned)up((size_t)(a.tiles_v * a.tiles_t), 8));
+
+	if (tile_t == 64)
+		hipLaunchKernelGGL((head_logits_kernel<64, MODE>), grid, dim3(kHeadThreads), 0, st, a);
+	else if (tile_t == 128)
+		hipLaunchKernelGGL((head_logits_kernel<128, MODE>), grid, dim3(kHeadThreads), 0, st, a);
+	else
+		hipLaunchKernelGGL((head_logits_kernel<256, MODE>), grid, dim3(kHeadThreads), 0, st, a);
+}
+
+static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
+{
+	hipStream_t st = compute_stream();
+	char *work = (char *)j.d_work;
+	uint16_t *xs = (uint16_t *)(work + p.off_xs);
+	int32_t *ts = (int32_t *)(work + p.off_ts);
+	float *lse = (float *)(work + p.off_lse);
+	const uint16_t *w = (const uint16_t *)j.d_w;
+	RowArgs ra;
+	LogitArgs la;
+	FinishArgs fa;
+
+	memset(&ra, 0, sizeof(ra));
+	ra.x = (const uint16_t *)j.d_x;
+	ra.ld_x = j.ld_x;
+	ra.target = j.d_target;
+	ra.rows = j.rows;
+	ra.rows_pad = p.rows_pad;
+	ra.d = j.d;
+	ra.d_pad = p.d_pad;
+	ra.vocab = j.vocab;
+	ra.vocab_pad = p.tiles_v * kSide;
+	ra.bias = j.d_bias;
+	ra.xs = xs;
+	ra.ts = ts;
+	ra.bs = (float *)(work + p.off_bs);
+	hipLaunchKernelGGL(head_rows_kernel, dim3(rows_grid(p.rows_pad * (p.d_pad / 8))), dim3(kThreads), 0, st, ra);
+
+	memset(&la, 0, sizeof(la));
+	la.w.part[0] = la.w.part[1] = w;
+	la.w.ld = (uint32_t)j.vocab;
+	la.w.rows = j.vocab;
+	la.w.depth = j.d;
+	la.x.part[0] = la.x.part[1] = xs;
+	la.x.ld = (uint32_t)p.d_pad;
+	la.x.rows = p.rows_pad;
+	la.x.depth = p.d_pad;
+	la.bias = ra.bs;
+	la.target = ts;
+	la.steps = (j.d + kStep - 1) / kStep;
+	la.tiles_v = p.tiles_v;
+	la.tiles_t = p.rows_pad / p.tile_t;
+	la.rows_pad = p.rows_pad;
+	la.part = (f32x2 *)(work + p.off_part);
+	la.target_logit = (float *)(work + p.off_hit);
+	logits_launch<kStats>(st, p.tile_t, la);
+
+	memset(&fa, 0, sizeof(fa));
+	fa.part = la.part;
+	fa.target_logit = la.target_logit;
+	fa.target = ts;
+	fa.tiles_v = p.tiles_v;
+	fa.rows = j.rows;
+	fa.rows_pad = p.rows_pad;
+	fa.lse = lse;
+	fa.nll = j.d_nll;
+	hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.rows_pad / 64)), dim3(kFinishWaves * 64), 0, st, fa);
+
+	for (int64_t v0 = 0; grad && v0 < j.vocab; v0 += p.piece) {
+		const int64_t left = j.vocab - v0;
+		const int64_t here = left < p.piece ? (int64_t)up((size_t)left, kSide) : p.piece;
+		uint16_t *delta = (uint16_t *)(work + p.off_delta);
+		uint16_t *low = delta + p.rows_pad * p.piece;
+		DxArgs xa;
+		DwArgs wa;
+
+		la.v0 = v0;
+		la.tiles_v = here / kSide;
+		la.lse = lse;
+		la.scale = (float)j.scale;
+		la.delta = delta;
+		la.delta_low = low;
+		la.ld_delta = p.piece;
+		if (p.parts == 2)
+			logits_launch<kDeltaPair>(st, p.tile_t, la);
+		else
+			logits_launch<kDelta>(st, p.tile_t, la);
+
+		memset(&wa, 0, sizeof(wa));
+		wa.x = la.x;
+		wa.x.rows = p.d_pad;
+		wa.x.depth = p.rows_pad;
+		wa.delta.part[0] = delta;
+		wa.delta.part[1] = low;
+		wa.delta.ld = (uint32_t)p.piece;
+		wa.delta.rows = here;
+		wa.delta.depth = p.rows_pad;
+		wa.steps = (int)(p.rows_pad / kStep);
+		wa.parts = p.parts;
+		wa.tiles_d = p.d_pad / kSide;
+		wa.tiles_v = here / kSide;
+		wa.d = j.d;
+		wa.vocab = j.vocab;
+		wa.v0 = v0;
+		wa.dw = j.d_dw;
+		wa.db = j.d_db;
+		const dim3 wgrid((unsigned)up((size_t)(wa.tiles_d * wa.tiles_v), 8));
+
+		if (j.d_dw) {
+			if (j.grad_type == ANNI_F32)
+				hipLaunchKernelGGL(head_dw_kernel<kF32>, wgrid, dim3(kHeadThreads), 0, st, wa);
+			else
+				hipLaunchKernelGGL(head_dw_kernel<kBF16>, wgrid, dim3(kHeadThreads), 0, st, wa);
+		}
+		if (j.d_db) {
+			DbArgs ba;
+
+			memset(&ba, 0, sizeof(ba));
+			ba.delta[0] = delta;
+			ba.delta[1] = low;
+			ba.parts = p.parts;
+			ba.ld = p.piece;
+			ba.rows_pad = p.rows_pad;
+			ba.v0 = v0;
+			ba.count = (int)(left < here ? left : here);
+			ba.db = j.d_db;
+			if (j.grad_type == ANNI_F32)
+				hipLaunchKernelGGL(head_db_kernel<kF32>, dim3((unsigned)(here / 64)), dim3(kHeadThreads), 0, st, ba);
+			else
+				hipLaunchKernelGGL(head_db_kernel<kBF16>, dim3((unsigned)(here / 64)), dim3(kHeadThreads), 0, st, ba);
+		}
+		if (j.d_dx) {
+			memset(&xa, 0, sizeof(xa));
+			xa.delta = wa.delta;
+			xa.delta.rows = p.rows_pad;
+			xa.delta.depth = here;
+			xa.w.part[0] = xa.w.part[1] = w + v0;
+			xa.w.ld = (uint32_t)j.vocab;
+			xa.w.rows = j.d;
+			xa.w.depth = left;
+			xa.steps = (int)((left < here ? left : here) + kStep - 1) / kStep;
+			xa.parts = p.parts;
+			xa.splits = p.splits;
+			xa.tiles_t = p.rows_pad / p.tile_t;
+			xa.tiles_d = p.d_pad / kSide;
+			xa.slot = (float *)(work + p.off_slot);
+			xa.rows_pad = p.rows_pad;
+			xa.d_pad = p.d_pad;
+			xa.add = v0 > 0;
+			const dim3 grid((unsigned)up((size_t)(xa.tiles_t * xa.tiles_d), 8), (unsigned)p.splits);
+
+			if (p.tile_t == 64)
+				hipLaunchKernelGGL(head_dx_kernel<64>, grid, dim3(kHeadThreads), 0, st, xa);
+			else if (p.tile_t == 128)
+				hipLaunchKernelGGL(head_dx_kernel<128>, grid, dim3(kHeadThreads), 0, st, xa);
+			else
+				hipLaunchKernelGGL(head_dx_kernel<256>, grid, dim3(kHeadThreads), 0, st, xa);
+		}
+	}
+	if (grad && j.d_dx) {
+		DxSumArgs sa;
+
+		memset(&sa, 0, sizeof(sa));
+		sa.slot = (const float *)(work + p.off_slot);
+		sa.splits = p.splits;
+		sa.rows = j.rows;
+		sa.rows_pad = p.rows_pad;
+		sa.d = j.d;
+		sa.d_pad = p.d_pad;
+		sa.dx = j.d_dx;
+		sa.ld_dx = j.ld_dx;
+		const dim3 grid((unsigned)rows_grid(j.rows * (p.d_pad / 4)));
+
+		if (j.grad_type == ANNI_F32)
+			hipLaunchKernelGGL(head_dx_sum_kernel<kF32>, grid, dim3(kThreads), 0, st, sa);
+		else
+			hipLaunchKernelGGL(head_dx_sum_kernel<kBF16>, grid, dim3(kThreads), 0, st, sa);
+	}
+	return hip_ok(hipGetLastError(), "head_loss") ? 0 : -1;
+}
+
+} /* namespace anni */
+
+using namespace anni;
+
+extern "C" {
+
+size_t anni_head_loss_work_bytes(int64_t rows, int d, int vocab, int grad_type)
+{
+	HeadPlan p;
+
+	return head_plan(rows, d, vocab, grad_type, &p) ? p.bytes : 0;
+}
+
+int anni_head_loss(const anni_head_job *job)
+{
+	HeadPlan p;
+	bool grad;
+	uintptr_t grad_mask;
+
+	if (!job || !job->d_x || !job->d_w || !job->d_target || !job->d_nll || !job->d_work)
+		return -1;
+	grad = job->d_dx || job->d_dw || job->d_db;
+	if (!head_plan(job->rows, job->d, job->vocab, grad ? job->grad_type : -1, &p) || job->ld_x < job->d
+	    || (job->d_dx && job->ld_dx < job->d) || job->work_bytes < p.bytes)
+		return -1;
+	/* an element starts where its type may; the work area is ours to lay out */
+	grad_mask = grad && job->grad_type == ANNI_F32 ? 3 : 1;
+	if ((((uintptr_t)job->d_x | (uintptr_t)job->d_w) & 1) != 0
+	    || (((uintptr_t)job->d_bias | (uintptr_t)job->d_target | (uintptr_t)job->d_nll) & 3) != 0
+	    || (((uintptr_t)job->d_dx | (uintptr_t)job->d_dw | (uintptr_t)job->d_db) & grad_mask) != 0
+	    || ((uintptr_t)job->d_work & 255) != 0)
+		return -1;
+	if (!device_ready())
+		return -1;
+	return head_run(*job, p, grad);
+}
+
+int anni_adam_head_loss(anni_adam *opt, int w_tensor, int b_tensor, const anni_head_job *job, int with_grad)
+{
+	anni_head_job j;
+	int64_t w_at, w_n, b_at = 0, b_n;
+
+	if (!opt || !opt->priv || !job || !opt->d_param_bf16 || job->d <= 0 || w_tensor < 0
+	    || w_tensor >= opt->n_tensors || b_tensor < -1 || b_tensor >= opt->n_tensors)
+		return -1;
+	w_at = anni_adam_tensor_offset(opt, w_tensor);
+	w_n = (w_tensor + 1 < opt->n_tensors ? anni_adam_tensor_offset(opt, w_tensor + 1) : opt->n) - w_at;
+	if (w_n <= 0 || w_n % job->d != 0 || w_n / job->d > kHeadMaxVocab)
+		return -1;
+	j = *job;
+	j.vocab = (int)(w_n / job->d);
+	j.d_w = (const uint16_t *)opt->d_param_bf16 + w_at;
+	j.d_bias = nullptr;
+	if (b_tensor >= 0) {
+		b_at = anni_adam_tensor_offset(opt, b_tensor);
+		b_n = (b_tensor + 1 < opt->n_tensors ? anni_adam_tensor_offset(opt, b_tensor + 1) : opt->n) - b_at;
+		if (b_n != j.vocab)
+			return -1;
+		j.d_bias = opt->d_param + b_at;
+	}
+	j.grad_type = opt->cfg.grad_type;
+	j.d_dw = nullptr;
+	j.d_db = nullptr;
+	if (with_grad) {
+		const size_t size = opt->cfg.grad_type == ANNI_F32 ? 4 : 2;
+
+		if (opt->cfg.grad_type == ANNI_FP8_E4M3 || !opt->d_grad)
+			return -1;
+		j.d_dw = (char *)opt->d_grad + (size_t)w_at * size;
+		if (b_tensor >= 0)
+			j.d_db = (char *)opt->d_grad + (size_t)b_at * size;
+	} else {
+		j.d_dx = nullptr;
+	}
+	return anni_head_loss(&j);
+}
+
+} /* extern "C" */

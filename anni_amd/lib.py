@@ -52,6 +52,16 @@ class Colsum(C.Structure):
                 ("rows", C.c_int64), ("cols", C.c_int)]
 
 
+class HeadJob(C.Structure):
+    """anni_head_job: one call of the head's loss."""
+    _fields_ = [("rows", C.c_int64), ("d", C.c_int), ("vocab", C.c_int), ("d_x", C.c_void_p),
+                ("ld_x", C.c_int64), ("d_w", C.c_void_p), ("d_bias", C.c_void_p),
+                ("d_target", C.c_void_p), ("d_nll", C.c_void_p), ("scale", C.c_double),
+                ("d_dx", C.c_void_p), ("ld_dx", C.c_int64), ("d_dw", C.c_void_p),
+                ("d_db", C.c_void_p), ("grad_type", C.c_int), ("d_work", C.c_void_p),
+                ("work_bytes", C.c_size_t)]
+
+
 class Pack(C.Structure):
     """anni_pack: a second home for the bf16 of a matrix inside a packed matrix."""
     _fields_ = [("tensor", C.c_int), ("cols", C.c_int32), ("dst_offset", C.c_int64),
@@ -130,6 +140,9 @@ _PROTOS = {
     "anni_f32_to_bf16": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64]),
     "anni_fp8_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
     "anni_colsum_add": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int]),
+    "anni_head_loss_work_bytes": (C.c_size_t, [C.c_int64, C.c_int, C.c_int, C.c_int]),
+    "anni_head_loss": (C.c_int, [C.POINTER(HeadJob)]),
+    "anni_adam_head_loss": (C.c_int, [C.POINTER(Adam), C.c_int, C.c_int, C.POINTER(HeadJob), C.c_int]),
     "anni_colsum_add_batch": (C.c_int, [C.POINTER(Colsum), C.c_int]),
 }
 

@@ -354,6 +354,61 @@ typedef struct anni_colsum {
 } anni_colsum;
 int	anni_colsum_add_batch(const anni_colsum *jobs, int n_jobs);
 
+/*
+** The head's loss: softmax cross entropy of logits = x w + b over the whole vocabulary, with its
+** gradients, without the logits in memory.  x is bf16 [rows][ld_x] (the last hidden states), w the
+** bf16 [d][vocab] matrix the step keeps as the twin of w_head (lang/lm.c's logits = h w_head + b_head), b float [vocab]
+** or NULL.
+**   nll[i] = log sum_v exp(l[i][v]) - l[i][target_i]
+**   delta[i][v] = scale * (exp(l[i][v] - lse_i) - [v == target_i])
+**   dx = delta w^T (overwritten),  dw += x^T delta,  db += column sums of delta
+** dw and db are added to, so they can point straight into the gradient flat (what earlier
+** microbatches left there stays; the step clears it); with scale = 1 / (B (T - 1)) they are the mean
+** loss's.  A row whose target is not in [0, vocab) takes no part: its nll is 0, its dx 0, and
+** whatever its x holds reaches nothing.  A logit of -inf has probability 0; a row with nothing else
+** has no distribution: NaN.
+**
+** Sums are float, products of bf16 numbers exact.  delta is rounded to bf16 for ANNI_BF16 gradients
+** and kept as a pair of bf16 numbers for ANNI_F32 (an error of 2^-17 of each element); db is summed
+** from the same numbers.  No atomics: a run repeats bit for bit.
+**
+** d_work: work_bytes of device memory, 256-byte aligned, at least anni_head_loss_work_bytes of the
+** same sizes; nothing is kept in it between calls, and calls on different streams (or recorded
+** into graphs that may run at the same time) need one each.  It holds a copy of x, and for the gradients one
+** piece of delta of at most 512 MiB (more only if 256 places of the vocabulary need it).  Nothing else is allocated and nothing waits for
+** the host.
+*/
+typedef struct anni_head_job {
+	int64_t		rows;		/* up to 2^22 */
+	int		d;		/* up to 2^16 */
+	int		vocab;		/* up to 2^22 */
+	const void	*d_x;		/* bf16 */
+	int64_t		ld_x;		/* >= d */
+	const void	*d_w;		/* bf16 */
+	const float	*d_bias;	/* may be NULL */
+	const int32_t	*d_target;
+	float		*d_nll;		/* [rows] */
+	double		scale;
+	void		*d_dx;		/* all three NULL: the loss alone; any of them may be */
+	int64_t		ld_dx;		/* >= d */
+	void		*d_dw;
+	void		*d_db;
+	int		grad_type;	/* ANNI_F32 or ANNI_BF16, of dx, dw and db */
+	void		*d_work;
+	size_t		work_bytes;
+} anni_head_job;
+/* grad_type -1: the loss alone.  0 for sizes or a type that are refused. */
+size_t	anni_head_loss_work_bytes(int64_t rows, int d, int vocab, int grad_type);
+int	anni_head_loss(const anni_head_job *job);
+/*
+** The same on an arena: w is the twin of tensor w_tensor (d * vocab elements, vocab from
+** b_tensor's or w_tensor's size and d), b the float values of b_tensor (-1: none), and dw and db go
+** into the bound gradient flat.  x, targets, nll, scale, dx and the work area come from `job`, whose
+** vocab, d_w, d_bias, d_dw, d_db and grad_type are not read.  with_grad == 0: the loss alone.
+** -1 for gradients in an arena whose gradients are E4M3 codes (their scales are known only afterwards), or without twins.
+*/
+int	anni_adam_head_loss(anni_adam *opt, int w_tensor, int b_tensor, const anni_head_job *job, int with_grad);
+
 #ifdef __cplusplus
 }
 #endif
