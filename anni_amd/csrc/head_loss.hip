@@ -40,54 +40,100 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 /* sixteen bytes at any element: rows of an odd vocabulary are not aligned (the hardware does not mind) */
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-constexpr int kHeadThreads = 512;	/* eight wavefronts, two to a SIMD */
 constexpr int kStep = 64;		/* of the contracted axis per trip */
 constexpr int kSide = 256;		/* of a result tile along the vocabulary or the model's width */
 
+#ifndef HEAD_T256
+#define HEAD_T256 512
+#endif
 #define ANNI_LDS __attribute__((address_space(3)))
 
 /*
 ** One operand of a product: element (r, k), 0 <= r < ROWS of the tile, k of a step.  BY_ROW: the
-** rows are contiguous (element (r, k) at k ld + r), else the contracted axis (r ld + k).  CHECK: the
-** array ends inside tiles; loads never leave it: what lies beyond along the contiguous axis reads as
-** 0, beyond along the other one the last valid line again (its product is with zeros, or not kept).
-** LDS image: 16-byte chunks, those of a line rotated by an exclusive or so that the lanes of a
-** fragment read spread over all banks.
+** rows are contiguous (element (r, k) at k ld + r), else the contracted axis (r ld + k).
+**
+** Its image in LDS is a list of 16-byte chunks in the order the lanes of a workgroup name them, so
+** that a load can put them there itself, past the registers; a line's chunks are permuted by an
+** exclusive or with its index (on the side of the memory address), so that the lanes of a fragment
+** read spread over all banks.
+**
+** CHECK: the array ends inside tiles or its lines are not aligned to 16 bytes; such tiles go through
+** registers.  Loads never leave the array: what lies beyond along the contiguous axis reads as 0,
+** beyond along the other one the last valid line again (its product is with zeros, or not kept).
 */
 struct Source {
 	const uint16_t	*part[2];	/* second: the low halves, same shape */
 	uint32_t	ld;
 	int64_t		rows;		/* valid rows from row 0 */
 	int64_t		depth;		/* valid length of the contracted axis */
+	int		aligned;	/* every chunk is 16-byte aligned */
 };
 
-template <bool BY_ROW, bool CHECK, int ROWS>
-struct Operand {
-	static constexpr int kChunks = ROWS * kStep / 8 / kHeadThreads;
-	static constexpr int kBytes = ROWS * kStep * 2;
-	u32x4	hold[kChunks];
+/*
+** Sixteen bytes per lane from base + offset to 16 l behind `lds` (both uniform but the offset).  In
+** assembly because behind the builtin the compiler waits for every such load before any read of LDS,
+** and this one's whole point is to stay on its way; arrived() is the wait, before the barrier that
+** hands the data over.  It writes no register, and loads of the compiler's own only ever wait for more
+** than they must (they return in order).  m0 must have been written one instruction before its use.
+*/
+__device__ __forceinline__ void memory_to_lds(const uint16_t *base, uint32_t offset, char *lds)
+{
+	const uint32_t at = (uint32_t)(uintptr_t)(ANNI_LDS char *)lds;
 
-	/* step `s` of `steps` per part */
-	__device__ __forceinline__ void fetch(const Source &src, int64_t row0, int s, int steps, int tid)
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+	    : : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(base) : "memory");
+}
+
+__device__ __forceinline__ void arrived(void)
+{
+	asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+}
+
+template <bool BY_ROW, bool CHECK, int ROWS, int THREADS>
+struct Operand {
+	static constexpr int kChunks = ROWS * kStep / 8 / THREADS;
+	static constexpr int kBytes = ROWS * kStep * 2;
+	static constexpr int kLine = BY_ROW ? ROWS / 8 : kStep / 8;	/* chunks to a line */
+	u32x4	hold[CHECK ? kChunks : 1];
+	bool	held;
+
+	static __device__ __forceinline__ int turn(int line)
+	{
+		return BY_ROW ? (line & 3) << 2 : line & 7;
+	}
+
+	/* Step `s` (of `steps` per part) on its way to `lds`, or into registers. */
+	__device__ __forceinline__ void start(const Source &src, int64_t row0, int s, int steps, char *lds, int tid)
 	{
 		const int part = s >= steps ? 1 : 0;
 		const int64_t k0 = (int64_t)(s - part * steps) * kStep;
 		const uint16_t *base = src.part[part] + (BY_ROW ? k0 * src.ld + row0 : row0 * src.ld + k0);
 		const int64_t rows_left = src.rows - row0;
 		const int64_t depth_left = src.depth - k0;
-		const bool inside = !CHECK || (rows_left >= ROWS && depth_left >= kStep);
+
+		held = CHECK && (rows_left < ROWS || depth_left < kStep || !src.aligned);
+		if (!CHECK || !held) {
+			const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
 #pragma unroll
-		for (int i = 0; i < kChunks; i++) {
-			const int c = tid + i * kHeadThreads;
-			const int line = BY_ROW ? c / (ROWS / 8) : c / (kStep / 8);
-			const int col = (BY_ROW ? c % (ROWS / 8) : c % (kStep / 8)) * 8;
+			for (int i = 0; i < kChunks; i++) {
+				const int c = tid + i * THREADS;
+				const int line = c / kLine;
+				const int chunk = (c % kLine) ^ turn(line);
 
-			if (inside) {
-				hold[i] = *(const u32x4_any *)(base + ((uint32_t)line * src.ld + (uint32_t)col));
-			} else {
-				const int64_t lines = BY_ROW ? depth_left : rows_left;
-				const int64_t cols = BY_ROW ? rows_left : depth_left;
+				memory_to_lds(base, ((uint32_t)line * src.ld + (uint32_t)chunk * 8) * 2, lds + (i * THREADS + wave * 64) * 16);
+			}
+			return;
+		}
+		if constexpr (CHECK) {
+			const int64_t lines = BY_ROW ? depth_left : rows_left;
+			const int64_t cols = BY_ROW ? rows_left : depth_left;
+
+#pragma unroll
+			for (int i = 0; i < kChunks; i++) {
+				const int c = tid + i * THREADS;
+				const int line = c / kLine;
+				const int col = ((c % kLine) ^ turn(line)) * 8;
 				const uint16_t *p = base + (uint32_t)(line < lines ? line : (int)lines - 1) * src.ld;
 				u32x4 w = {0u, 0u, 0u, 0u};
 
@@ -110,23 +156,20 @@ struct Operand {
 		}
 	}
 
-	static __device__ __forceinline__ uint32_t place(int line, int chunk)
+	/* What start() left in registers goes to `lds`. */
+	__device__ __forceinline__ void finish(char *lds, int tid) const
 	{
-		if (BY_ROW)
-			return (uint32_t)line * (ROWS * 2) + (uint32_t)((chunk ^ ((line & 3) << 2)) * 16);
-		return (uint32_t)line * (kStep * 2) + (uint32_t)((chunk ^ (line & 7)) * 16);
+		if constexpr (CHECK) {
+			if (held)
+#pragma unroll
+				for (int i = 0; i < kChunks; i++)
+					*(u32x4 *)(lds + (tid + i * THREADS) * 16) = hold[i];
+		}
 	}
 
-	__device__ __forceinline__ void put(char *lds, int tid) const
+	static __device__ __forceinline__ uint32_t place(int line, int chunk)
 	{
-#pragma unroll
-		for (int i = 0; i < kChunks; i++) {
-			const int c = tid + i * kHeadThreads;
-			const int line = BY_ROW ? c / (ROWS / 8) : c / (kStep / 8);
-			const int chunk = BY_ROW ? c % (ROWS / 8) : c % (kStep / 8);
-
-			*(u32x4 *)(lds + place(line, chunk)) = hold[i];
-		}
+		return (uint32_t)(line * kLine + (chunk ^ turn(line))) * 16;
 	}
 
 	/* Fragment of a 32 x 32 x 16 product: lane l holds row r0 + l % 32, places 16 sub + 8 (l / 32) .. + 7. */
@@ -148,57 +191,122 @@ struct Operand {
 	}
 };
 
-/* acc += A B^T over the steps [from, to): acc[i][j] is the 32 x 32 block (i, j) of the wavefront's part. */
+/*
+** acc += A B^T over the steps [from, to): acc[i][j] is the 32 x 32 block (i, j) of the wavefront's part.
+**
+** A step's operands are on their way into one half of LDS while the other half is computed on, and
+** the fragments of a 16-deep slice are read while the slice before is multiplied.  The one barrier
+** of a step stands before its last slice's products, whose fragments are in registers by then: behind
+** it the first fragments of the next step are read under those products, and the half that everyone
+** has read is filled again.  lds[0] and lds[1] are arrays of their own: the compiler then knows that
+** reading one does not wait for what is on its way into the other.
+*/
 template <class A, class B, int MB, int NB>
-__device__ __forceinline__ void product(f32x16 (&acc)[MB][NB], const Source &sa, const Source &sb, int64_t row_a,
-	int64_t row_b, int from, int to, int steps, char *lds, int ra, int rb, int tid)
-{
-	A a;
-	B b;
-	const int lane = tid & 63;
-	constexpr int kBuffer = A::kBytes + B::kBytes;
-	int at = 0;
+struct Product {
+	f32x16	acc[MB][NB];
 
-	if (from >= to)
-		return;		/* an empty slice; the same in every lane of the workgroup */
-	a.fetch(sa, row_a, from, steps, tid);
-	b.fetch(sb, row_b, from, steps, tid);
-	a.put(lds, tid);
-	b.put(lds + A::kBytes, tid);
-	__syncthreads();
-	for (int s = from; s < to; s++) {
-		const char *la = lds + at * kBuffer;
-		const char *lb = la + A::kBytes;
-
-		if (s + 1 < to) {
-			a.fetch(sa, row_a, s + 1, steps, tid);
-			b.fetch(sb, row_b, s + 1, steps, tid);
-		}
+	__device__ __forceinline__ void clear(void)
+	{
 #pragma unroll
-		for (int sub = 0; sub < kStep / 16; sub++) {
-			bf16x8 fa[MB], fb[NB];
-
-#pragma unroll
-			for (int i = 0; i < MB; i++)
-				fa[i] = A::fragment(la, ra + i * 32, sub, lane);
+		for (int i = 0; i < MB; i++)
 #pragma unroll
 			for (int j = 0; j < NB; j++)
-				fb[j] = B::fragment(lb, rb + j * 32, sub, lane);
+				acc[i][j] = f32x16{};
+	}
+
+	struct Slice {
+		bf16x8	a[MB], b[NB];
+	};
+
+	static __device__ __forceinline__ void read(Slice &f, const char *la, const char *lb, int ra, int rb, int sub,
+		int lane)
+	{
 #pragma unroll
-			for (int i = 0; i < MB; i++)
+		for (int i = 0; i < MB; i++)
+			f.a[i] = A::fragment(la, ra + i * 32, sub, lane);
 #pragma unroll
-				for (int j = 0; j < NB; j++)
-					acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+		for (int j = 0; j < NB; j++)
+			f.b[j] = B::fragment(lb, rb + j * 32, sub, lane);
+	}
+
+	__device__ __forceinline__ void multiply(const Slice &f)
+	{
+#pragma unroll
+		for (int i = 0; i < MB; i++)
+#pragma unroll
+			for (int j = 0; j < NB; j++)
+				acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
+	}
+
+	struct Where {
+		const Source	*a, *b;
+		int64_t		row_a, row_b;
+		int		to, steps, ra, rb, tid;
+	};
+
+	/* Step s lies in `here`, its first slice in f0; s + 1 goes to `next`. */
+	__device__ __forceinline__ void step(const Where &w, int s, char *here_a, char *here_b, char *next_a,
+		char *next_b, Slice &f0, Slice &f1)
+	{
+		const int lane = w.tid & 63;
+		const bool more = s + 1 < w.to;
+		A a;
+		B b;
+
+		static_assert(kStep == 64, "four slices");
+		if (more) {
+			a.start(*w.a, w.row_a, s + 1, w.steps, next_a, w.tid);
+			b.start(*w.b, w.row_b, s + 1, w.steps, next_b, w.tid);
 		}
-		if (s + 1 < to) {
-			/* the other buffer: its last readers passed the barrier at the end of the step before */
-			at ^= 1;
-			a.put(lds + at * kBuffer, tid);
-			b.put(lds + at * kBuffer + A::kBytes, tid);
+		read(f1, here_a, here_b, w.ra, w.rb, 1, lane);
+		multiply(f0);
+		__builtin_amdgcn_sched_barrier(0);
+		read(f0, here_a, here_b, w.ra, w.rb, 2, lane);
+		multiply(f1);
+		__builtin_amdgcn_sched_barrier(0);
+		read(f1, here_a, here_b, w.ra, w.rb, 3, lane);
+		multiply(f0);
+		__builtin_amdgcn_sched_barrier(0);
+		if (more) {
+			a.finish(next_a, w.tid);
+			b.finish(next_b, w.tid);
+			arrived();
 		}
 		__syncthreads();
+		if (more)
+			read(f0, next_a, next_b, w.ra, w.rb, 0, lane);
+		multiply(f1);
+		__builtin_amdgcn_sched_barrier(0);
 	}
-}
+
+	__device__ __forceinline__ void run(const Source &sa, const Source &sb, int64_t row_a, int64_t row_b, int from,
+		int to, int steps, char *a0, char *b0, char *a1, char *b1, int ra, int rb, int tid)
+	{
+		const Where w = { &sa, &sb, row_a, row_b, to, steps, ra, rb, tid };
+		Slice f0, f1;
+
+		clear();
+		if (from >= to)
+			return;		/* an empty slice of the axis; the same in every lane of the workgroup */
+		{
+			A a;
+			B b;
+
+			a.start(sa, row_a, from, steps, a0, tid);
+			b.start(sb, row_b, from, steps, b0, tid);
+			a.finish(a0, tid);
+			b.finish(b0, tid);
+			arrived();
+		}
+		__syncthreads();
+		read(f0, a0, b0, ra, rb, 0, tid & 63);
+		for (int s = from; s < to; s += 2) {
+			step(w, s, a0, b0, a1, b1, f0, f1);
+			if (s + 1 < to)
+				step(w, s + 1, a1, b1, a0, b0, f0, f1);
+		}
+	}
+};
 
 /* Row of register r of a 32 x 32 block in lane l; the column is l % 32. */
 __device__ __forceinline__ int block_row(int r, int lane)
@@ -304,22 +412,31 @@ struct LogitArgs {
 
 enum { kStats = 0, kDelta = 1, kDeltaPair = 2 };
 
-template <int TT> struct LogitWaves { static constexpr int m = TT == 256 ? 2 : TT == 128 ? 4 : 8, n = 8 / m; };
+/*
+** Wavefronts of a workgroup for tiles of TT tokens, and how they share the tile: kWavesM along the
+** product's first axis.
+*/
+template <int TT> struct Shape {
+	static constexpr int threads = TT == 256 ? HEAD_T256 : 512;
+	static constexpr int waves = threads / 64;
+};
 
 template <int TT, int MODE>
-__global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
+__global__ __launch_bounds__(Shape<TT>::threads) void head_logits_kernel(LogitArgs a)
 {
-	typedef Operand<true, true, kSide> W;
-	typedef Operand<false, false, TT> X;
-	constexpr int WM = LogitWaves<TT>::m, WN = LogitWaves<TT>::n;
+	constexpr int kHeadThreads = Shape<TT>::threads;
+	constexpr int WM = TT == 256 ? 2 : TT == 128 ? 4 : 8, WN = Shape<TT>::waves / WM;
+	typedef Operand<true, true, kSide, kHeadThreads> W;
+	typedef Operand<false, false, TT, kHeadThreads> X;
 	constexpr int MB = kSide / WM / 32, NB = TT / WN / 32;
-	__shared__ __align__(16) char lds[2 * (W::kBytes + X::kBytes)];
+	__shared__ __align__(16) char lw0[W::kBytes], lx0[X::kBytes], lw1[W::kBytes], lx1[X::kBytes];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	int64_t tv, tt;
-	f32x16 acc[MB][NB];
+	Product<W, X, MB, NB> prod;
+	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_t, &tv, &tt))
 		return;
@@ -327,13 +444,7 @@ __global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
 	const int64_t t_tile = tt * TT;
 	const int64_t v_base = v_tile + wm * (MB * 32);
 
-#pragma unroll
-	for (int i = 0; i < MB; i++)
-#pragma unroll
-		for (int j = 0; j < NB; j++)
-			acc[i][j] = f32x16{};
-	product<W, X, MB, NB>(acc, a.w, a.x, v_tile, t_tile, 0, a.steps, a.steps, lds, wm * (MB * 32), wn * (NB * 32),
-	    tid);
+	prod.run(a.w, a.x, v_tile, t_tile, 0, a.steps, a.steps, lw0, lx0, lw1, lx1, wm * (MB * 32), wn * (NB * 32), tid);
 #pragma unroll
 	for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -349,7 +460,7 @@ __global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
 				__builtin_amdgcn_sched_barrier(0);	/* all loads ahead of all sums take registers that there are not */
 		}
 	if constexpr (MODE == kStats) {
-		f32x2 *red = (f32x2 *)lds;	/* [WM][TT]; product() ended with a barrier */
+		f32x2 *red = (f32x2 *)lw0;	/* [WM][TT]; every wavefront's last read lies before the last step's barrier */
 
 #pragma unroll
 		for (int j = 0; j < NB; j++) {
@@ -503,13 +614,14 @@ struct DxArgs {
 
 /* One slice of the contracted axis (the vocabulary) per blockIdx.y, each with a slot of its own. */
 template <int TT>
-__global__ __launch_bounds__(kHeadThreads) void head_dx_kernel(DxArgs a)
+__global__ __launch_bounds__(Shape<TT>::threads) void head_dx_kernel(DxArgs a)
 {
-	typedef Operand<false, false, TT> D;
-	typedef Operand<false, true, kSide> W;
-	constexpr int WM = 2, WN = 4;
+	constexpr int kHeadThreads = Shape<TT>::threads;
+	constexpr int WM = 2, WN = Shape<TT>::waves / WM;
+	typedef Operand<false, false, TT, kHeadThreads> D;
+	typedef Operand<false, true, kSide, kHeadThreads> W;
 	constexpr int MB = TT / WM / 32, NB = kSide / WN / 32;
-	__shared__ __align__(16) char lds[2 * (D::kBytes + W::kBytes)];
+	__shared__ __align__(16) char ld0[D::kBytes], lw0[W::kBytes], ld1[D::kBytes], lw1[W::kBytes];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -518,17 +630,13 @@ __global__ __launch_bounds__(kHeadThreads) void head_dx_kernel(DxArgs a)
 	const int from = (int)((int64_t)total * blockIdx.y / a.splits);
 	const int to = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
 	int64_t tt, td;
-	f32x16 acc[MB][NB];
+	Product<D, W, MB, NB> prod;
+	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_t, a.tiles_d, &tt, &td))
 		return;
-#pragma unroll
-	for (int i = 0; i < MB; i++)
-#pragma unroll
-		for (int j = 0; j < NB; j++)
-			acc[i][j] = f32x16{};
-	product<D, W, MB, NB>(acc, a.delta, a.w, tt * TT, td * kSide, from, to, a.steps, lds, wm * (MB * 32),
-	    wn * (NB * 32), tid);
+	prod.run(a.delta, a.w, tt * TT, td * kSide, from, to, a.steps, ld0, lw0, ld1, lw1, wm * (MB * 32), wn * (NB * 32),
+	    tid);
 #pragma unroll
 	for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -602,29 +710,26 @@ __device__ __forceinline__ void add_to(void *base, int64_t i, float x)
 }
 
 template <int GT>
-__global__ __launch_bounds__(kHeadThreads) void head_dw_kernel(DwArgs a)
+__global__ __launch_bounds__(Shape<256>::threads) void head_dw_kernel(DwArgs a)
 {
-	typedef Operand<true, false, kSide> X;
-	typedef Operand<true, false, kSide> D;
-	constexpr int WM = 2, WN = 4;
+	constexpr int kHeadThreads = Shape<256>::threads;
+	constexpr int WM = 2, WN = Shape<256>::waves / WM;
+	typedef Operand<true, false, kSide, kHeadThreads> X;
+	typedef Operand<true, false, kSide, kHeadThreads> D;
 	constexpr int MB = kSide / WM / 32, NB = kSide / WN / 32;
-	__shared__ __align__(16) char lds[2 * (X::kBytes + D::kBytes)];
+	__shared__ __align__(16) char lx0[X::kBytes], ld0[D::kBytes], lx1[X::kBytes], ld1[D::kBytes];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	int64_t td, tv;
-	f32x16 acc[MB][NB];
+	Product<X, D, MB, NB> prod;
+	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_d, &tv, &td))
 		return;
-#pragma unroll
-	for (int i = 0; i < MB; i++)
-#pragma unroll
-		for (int j = 0; j < NB; j++)
-			acc[i][j] = f32x16{};
-	product<X, D, MB, NB>(acc, a.x, a.delta, td * kSide, tv * kSide, 0, a.steps * a.parts, a.steps, lds,
-	    wm * (MB * 32), wn * (NB * 32), tid);
+	prod.run(a.x, a.delta, td * kSide, tv * kSide, 0, a.steps * a.parts, a.steps, lx0, ld0, lx1, ld1, wm * (MB * 32),
+	    wn * (NB * 32), tid);
 #pragma unroll
 	for (int j = 0; j < NB; j++) {
 		const int64_t v = a.v0 + tv * kSide + wn * (NB * 32) + j * 32 + (lane & 31);
@@ -654,7 +759,7 @@ struct DbArgs {
 
 /* db += column sums of delta: 64 columns to a workgroup, rows shared by its wavefronts, fixed order. */
 template <int GT>
-__global__ __launch_bounds__(kHeadThreads) void head_db_kernel(DbArgs a)
+__global__ __launch_bounds__(512) void head_db_kernel(DbArgs a)
 {
 	__shared__ float red[8][64];
 	const int lane = threadIdx.x & 63;
@@ -757,11 +862,11 @@ static void logits_launch(hipStream_t st, int tile_t, const LogitArgs &a)
 	const dim3 grid((unsigned)up((size_t)(a.tiles_v * a.tiles_t), 8));
 
 	if (tile_t == 64)
-		hipLaunchKernelGGL((head_logits_kernel<64, MODE>), grid, dim3(kHeadThreads), 0, st, a);
+		hipLaunchKernelGGL((head_logits_kernel<64, MODE>), grid, dim3(Shape<64>::threads), 0, st, a);
 	else if (tile_t == 128)
-		hipLaunchKernelGGL((head_logits_kernel<128, MODE>), grid, dim3(kHeadThreads), 0, st, a);
+		hipLaunchKernelGGL((head_logits_kernel<128, MODE>), grid, dim3(Shape<128>::threads), 0, st, a);
 	else
-		hipLaunchKernelGGL((head_logits_kernel<256, MODE>), grid, dim3(kHeadThreads), 0, st, a);
+		hipLaunchKernelGGL((head_logits_kernel<256, MODE>), grid, dim3(Shape<256>::threads), 0, st, a);
 }
 
 static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
@@ -797,6 +902,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	la.w.ld = (uint32_t)j.vocab;
 	la.w.rows = j.vocab;
 	la.w.depth = j.d;
+	la.w.aligned = ((uintptr_t)w & 15) == 0 && j.vocab % 8 == 0;
 	la.x.part[0] = la.x.part[1] = xs;
 	la.x.ld = (uint32_t)p.d_pad;
 	la.x.rows = p.rows_pad;
@@ -864,9 +970,9 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 
 		if (j.d_dw) {
 			if (j.grad_type == ANNI_F32)
-				hipLaunchKernelGGL(head_dw_kernel<kF32>, wgrid, dim3(kHeadThreads), 0, st, wa);
+				hipLaunchKernelGGL(head_dw_kernel<kF32>, wgrid, dim3(Shape<256>::threads), 0, st, wa);
 			else
-				hipLaunchKernelGGL(head_dw_kernel<kBF16>, wgrid, dim3(kHeadThreads), 0, st, wa);
+				hipLaunchKernelGGL(head_dw_kernel<kBF16>, wgrid, dim3(Shape<256>::threads), 0, st, wa);
 		}
 		if (j.d_db) {
 			DbArgs ba;
@@ -881,9 +987,9 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			ba.count = (int)(left < here ? left : here);
 			ba.db = j.d_db;
 			if (j.grad_type == ANNI_F32)
-				hipLaunchKernelGGL(head_db_kernel<kF32>, dim3((unsigned)(here / 64)), dim3(kHeadThreads), 0, st, ba);
+				hipLaunchKernelGGL(head_db_kernel<kF32>, dim3((unsigned)(here / 64)), dim3(512), 0, st, ba);
 			else
-				hipLaunchKernelGGL(head_db_kernel<kBF16>, dim3((unsigned)(here / 64)), dim3(kHeadThreads), 0, st, ba);
+				hipLaunchKernelGGL(head_db_kernel<kBF16>, dim3((unsigned)(here / 64)), dim3(512), 0, st, ba);
 		}
 		if (j.d_dx) {
 			memset(&xa, 0, sizeof(xa));
@@ -894,6 +1000,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			xa.w.ld = (uint32_t)j.vocab;
 			xa.w.rows = j.d;
 			xa.w.depth = left;
+			xa.w.aligned = la.w.aligned;	/* v0 is a multiple of kSide */
 			xa.steps = (int)((left < here ? left : here) + kStep - 1) / kStep;
 			xa.parts = p.parts;
 			xa.splits = p.splits;
@@ -906,11 +1013,11 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			const dim3 grid((unsigned)up((size_t)(xa.tiles_t * xa.tiles_d), 8), (unsigned)p.splits);
 
 			if (p.tile_t == 64)
-				hipLaunchKernelGGL(head_dx_kernel<64>, grid, dim3(kHeadThreads), 0, st, xa);
+				hipLaunchKernelGGL(head_dx_kernel<64>, grid, dim3(Shape<64>::threads), 0, st, xa);
 			else if (p.tile_t == 128)
-				hipLaunchKernelGGL(head_dx_kernel<128>, grid, dim3(kHeadThreads), 0, st, xa);
+				hipLaunchKernelGGL(head_dx_kernel<128>, grid, dim3(Shape<128>::threads), 0, st, xa);
 			else
-				hipLaunchKernelGGL(head_dx_kernel<256>, grid, dim3(kHeadThreads), 0, st, xa);
+				hipLaunchKernelGGL(head_dx_kernel<256>, grid, dim3(Shape<256>::threads), 0, st, xa);
 		}
 	}
 	if (grad && j.d_dx) {
