@@ -40,12 +40,11 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 /* sixteen bytes at any element: rows of an odd vocabulary are not aligned (the hardware does not mind) */
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
+constexpr int kHeadWaves = 8;		/* two to a SIMD */
+constexpr int kHeadThreads = kHeadWaves * 64;
 constexpr int kStep = 64;		/* of the contracted axis per trip */
 constexpr int kSide = 256;		/* of a result tile along the vocabulary or the model's width */
 
-#ifndef HEAD_T256
-#define HEAD_T256 512
-#endif
 #define ANNI_LDS __attribute__((address_space(3)))
 
 /*
@@ -89,17 +88,29 @@ __device__ __forceinline__ void arrived(void)
 	asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
 }
 
-template <bool BY_ROW, bool CHECK, int ROWS, int THREADS>
+/* One lane's place in an operand: kept across the steps, all else is uniform (registers are what is short). */
+template <bool BY_ROW, bool CHECK, int ROWS>
 struct Operand {
-	static constexpr int kChunks = ROWS * kStep / 8 / THREADS;
+	static constexpr int kChunks = ROWS * kStep / 8 / kHeadThreads;
 	static constexpr int kBytes = ROWS * kStep * 2;
 	static constexpr int kLine = BY_ROW ? ROWS / 8 : kStep / 8;	/* chunks to a line */
-	u32x4	hold[CHECK ? kChunks : 1];
-	bool	held;
+	static constexpr int kApart = kHeadThreads / kLine;		/* lines between two chunks of a lane */
+	uint32_t	offset;		/* elements from the tile's start to the lane's first chunk */
+	int		line, col;	/* its line, and its place in it */
+	u32x4		hold[CHECK ? kChunks : 1];
+	bool		held;
 
 	static __device__ __forceinline__ int turn(int line)
 	{
 		return BY_ROW ? (line & 3) << 2 : line & 7;
+	}
+
+	__device__ __forceinline__ void init(const Source &src, int tid)
+	{
+		static_assert(kApart % 8 == 0, "turn() is the same for all chunks of a lane");
+		line = tid / kLine;
+		col = ((tid % kLine) ^ turn(line)) * 8;
+		offset = (uint32_t)line * src.ld + (uint32_t)col;
 	}
 
 	/* Step `s` (of `steps` per part) on its way to `lds`, or into registers. */
@@ -116,34 +127,30 @@ struct Operand {
 			const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
 #pragma unroll
-			for (int i = 0; i < kChunks; i++) {
-				const int c = tid + i * THREADS;
-				const int line = c / kLine;
-				const int chunk = (c % kLine) ^ turn(line);
-
-				memory_to_lds(base, ((uint32_t)line * src.ld + (uint32_t)chunk * 8) * 2, lds + (i * THREADS + wave * 64) * 16);
-			}
+			for (int i = 0; i < kChunks; i++)
+				memory_to_lds(base + (int64_t)(i * kApart) * src.ld, offset * 2,
+				    lds + (i * kHeadThreads + wave * 64) * 16);
 			return;
 		}
 		if constexpr (CHECK) {
-			const int64_t lines = BY_ROW ? depth_left : rows_left;
-			const int64_t cols = BY_ROW ? rows_left : depth_left;
+			const int lines = (int)(BY_ROW ? (depth_left < kStep ? depth_left : kStep)
+			    : (rows_left < ROWS ? rows_left : ROWS));
+			const int cols = (int)(BY_ROW ? (rows_left < ROWS ? rows_left : ROWS)
+			    : (depth_left < kStep ? depth_left : kStep));
 
 #pragma unroll
 			for (int i = 0; i < kChunks; i++) {
-				const int c = tid + i * THREADS;
-				const int line = c / kLine;
-				const int col = ((c % kLine) ^ turn(line)) * 8;
-				const uint16_t *p = base + (uint32_t)(line < lines ? line : (int)lines - 1) * src.ld;
+				const int at = line + i * kApart;
+				const uint16_t *q = base + (uint32_t)(at < lines ? at : lines - 1) * src.ld + (uint32_t)col;
 				u32x4 w = {0u, 0u, 0u, 0u};
 
 				if (col + 8 <= cols) {
-					w = *(const u32x4_any *)(p + col);
+					w = *(const u32x4_any *)q;
 				} else {
 					/* from the last element down, each pushing the others up */
 #pragma unroll 1
 					for (int j = 7; j >= 0; j--) {
-						const uint32_t e = col + j < cols ? p[col + j] : 0u;
+						const uint32_t e = col + j < cols ? q[j] : 0u;
 
 						w.w = (w.w << 16) | (w.z >> 16);
 						w.z = (w.z << 16) | (w.y >> 16);
@@ -163,32 +170,64 @@ struct Operand {
 			if (held)
 #pragma unroll
 				for (int i = 0; i < kChunks; i++)
-					*(u32x4 *)(lds + (tid + i * THREADS) * 16) = hold[i];
+					*(u32x4 *)(lds + (tid + i * kHeadThreads) * 16) = hold[i];
 		}
 	}
 
-	static __device__ __forceinline__ uint32_t place(int line, int chunk)
-	{
-		return (uint32_t)(line * kLine + (chunk ^ turn(line))) * 16;
-	}
+	/*
+	** Where a lane reads its fragments of BLOCKS blocks of 32 rows from row r0 on.  A fragment of a
+	** 32 x 32 x 16 product: lane l holds row l % 32 of the block, places 16 sub + 8 (l / 32) .. + 7.
+	** What the exclusive or touches needs an address of its own (by row: the block; else: the slice),
+	** the rest is a constant distance.
+	*/
+	template <int BLOCKS>
+	struct Reader {
+		ANNI_LDS const char *at[BY_ROW ? BLOCKS : kStep / 16];
 
-	/* Fragment of a 32 x 32 x 16 product: lane l holds row r0 + l % 32, places 16 sub + 8 (l / 32) .. + 7. */
-	static __device__ __forceinline__ bf16x8 fragment(const char *lds, int r0, int sub, int lane)
-	{
-		if constexpr (BY_ROW) {
-			/* each 16 lanes read four lines of 16 rows and get them turned: a lane one row of four lines */
-			const int line = sub * 16 + (lane >> 5) * 8 + ((lane & 15) >> 2);
-			const int row = r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-			const uint32_t half = (uint32_t)(row & 4) * 2;
-			union { i16x4 h[2]; bf16x8 f; } u;
+		__device__ __forceinline__ void init(const char *lds, int r0, int lane)
+		{
+			ANNI_LDS const char *base = (ANNI_LDS const char *)lds;
 
-			u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ANNI_LDS i16x4 *)(lds + place(line, row >> 3) + half));
-			u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ANNI_LDS i16x4 *)(lds + place(line + 4, row >> 3) + half));
-			return u.f;
-		} else {
-			return *(const bf16x8 *)(lds + place(r0 + (lane & 31), sub * 2 + (lane >> 5)));
+			if constexpr (BY_ROW) {
+				/* each 16 lanes read four lines of 16 rows and get them turned: a lane one row of four lines */
+				const int ln = (lane >> 5) * 8 + ((lane & 15) >> 2);
+
+#pragma unroll
+				for (int i = 0; i < BLOCKS; i++) {
+					const int row = r0 + i * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+
+					at[i] = base + ln * kLine * 16 + ((row >> 3) ^ turn(ln)) * 16 + (row & 4) * 2;
+				}
+			} else {
+				const int row = r0 + (lane & 31);
+
+#pragma unroll
+				for (int sub = 0; sub < kStep / 16; sub++)
+					at[sub] = base + row * kLine * 16 + ((sub * 2 + (lane >> 5)) ^ turn(row)) * 16;
+			}
 		}
-	}
+
+		__device__ __forceinline__ void move(int bytes)
+		{
+#pragma unroll
+			for (int i = 0; i < (BY_ROW ? BLOCKS : kStep / 16); i++)
+				at[i] += bytes;
+		}
+
+		__device__ __forceinline__ bf16x8 fragment(int block, int sub) const
+		{
+			if constexpr (BY_ROW) {
+				ANNI_LDS const char *q = at[block] + sub * 16 * kLine * 16;
+				union { i16x4 h[2]; bf16x8 f; } u;
+
+				u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ANNI_LDS i16x4 *)q);
+				u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ANNI_LDS i16x4 *)(q + 4 * kLine * 16));
+				return u.f;
+			} else {
+				return *(ANNI_LDS const bf16x8 *)(at[sub] + block * 32 * kLine * 16);
+			}
+		}
+	};
 };
 
 /*
@@ -198,12 +237,22 @@ struct Operand {
 ** the fragments of a 16-deep slice are read while the slice before is multiplied.  The one barrier
 ** of a step stands before its last slice's products, whose fragments are in registers by then: behind
 ** it the first fragments of the next step are read under those products, and the half that everyone
-** has read is filled again.  lds[0] and lds[1] are arrays of their own: the compiler then knows that
-** reading one does not wait for what is on its way into the other.
+** has read is filled again.
+**
+** SUMS: on request also sum[j] = the sums of B's rows over the contracted axis (every register of a
+** lane the same), by products with ones: two more matrix instructions to eight.
 */
-template <class A, class B, int MB, int NB>
+template <class A, class B, int MB, int NB, bool SUMS>
 struct Product {
 	f32x16	acc[MB][NB];
+	f32x16	sum[SUMS ? NB : 1];
+
+	struct Slice {
+		bf16x8	a[MB], b[NB];
+	};
+
+	typedef typename A::template Reader<MB> ReadA;
+	typedef typename B::template Reader<NB> ReadB;
 
 	__device__ __forceinline__ void clear(void)
 	{
@@ -212,25 +261,33 @@ struct Product {
 #pragma unroll
 			for (int j = 0; j < NB; j++)
 				acc[i][j] = f32x16{};
+		if constexpr (SUMS)
+#pragma unroll
+			for (int j = 0; j < NB; j++)
+				sum[j] = f32x16{};
 	}
 
-	struct Slice {
-		bf16x8	a[MB], b[NB];
-	};
-
-	static __device__ __forceinline__ void read(Slice &f, const char *la, const char *lb, int ra, int rb, int sub,
-		int lane)
+	static __device__ __forceinline__ void read(Slice &f, const ReadA &ra, const ReadB &rb, int sub)
 	{
 #pragma unroll
 		for (int i = 0; i < MB; i++)
-			f.a[i] = A::fragment(la, ra + i * 32, sub, lane);
+			f.a[i] = ra.fragment(i, sub);
 #pragma unroll
 		for (int j = 0; j < NB; j++)
-			f.b[j] = B::fragment(lb, rb + j * 32, sub, lane);
+			f.b[j] = rb.fragment(j, sub);
 	}
 
-	__device__ __forceinline__ void multiply(const Slice &f)
+	__device__ __forceinline__ void multiply(const Slice &f, bool sums)
 	{
+		if constexpr (SUMS)
+			if (sums) {
+				const u32x4 ones = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+
+#pragma unroll
+				for (int j = 0; j < NB; j++)
+					sum[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ones), f.b[j],
+					    sum[j], 0, 0, 0);
+			}
 #pragma unroll
 		for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -238,73 +295,67 @@ struct Product {
 				acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.a[i], f.b[j], acc[i][j], 0, 0, 0);
 	}
 
-	struct Where {
-		const Source	*a, *b;
-		int64_t		row_a, row_b;
-		int		to, steps, ra, rb, tid;
-	};
-
-	/* Step s lies in `here`, its first slice in f0; s + 1 goes to `next`. */
-	__device__ __forceinline__ void step(const Where &w, int s, char *here_a, char *here_b, char *next_a,
-		char *next_b, Slice &f0, Slice &f1)
+	/* ra, rb: the first row of the wavefront's part in the tiles. */
+	__device__ __forceinline__ void run(const Source &sa, const Source &sb, int64_t row_a, int64_t row_b, int from,
+		int to, int steps, char *lds, int ra, int rb, int tid, bool sums)
 	{
-		const int lane = w.tid & 63;
-		const bool more = s + 1 < w.to;
+		constexpr int kBuffer = A::kBytes + B::kBytes;
+		const int lane = tid & 63;
 		A a;
 		B b;
+		ReadA reada;
+		ReadB readb;
+		Slice f0, f1;
+		int next = kBuffer;		/* where the half for the next step begins */
 
 		static_assert(kStep == 64, "four slices");
-		if (more) {
-			a.start(*w.a, w.row_a, s + 1, w.steps, next_a, w.tid);
-			b.start(*w.b, w.row_b, s + 1, w.steps, next_b, w.tid);
-		}
-		read(f1, here_a, here_b, w.ra, w.rb, 1, lane);
-		multiply(f0);
-		__builtin_amdgcn_sched_barrier(0);
-		read(f0, here_a, here_b, w.ra, w.rb, 2, lane);
-		multiply(f1);
-		__builtin_amdgcn_sched_barrier(0);
-		read(f1, here_a, here_b, w.ra, w.rb, 3, lane);
-		multiply(f0);
-		__builtin_amdgcn_sched_barrier(0);
-		if (more) {
-			a.finish(next_a, w.tid);
-			b.finish(next_b, w.tid);
-			arrived();
-		}
-		__syncthreads();
-		if (more)
-			read(f0, next_a, next_b, w.ra, w.rb, 0, lane);
-		multiply(f1);
-		__builtin_amdgcn_sched_barrier(0);
-	}
-
-	__device__ __forceinline__ void run(const Source &sa, const Source &sb, int64_t row_a, int64_t row_b, int from,
-		int to, int steps, char *a0, char *b0, char *a1, char *b1, int ra, int rb, int tid)
-	{
-		const Where w = { &sa, &sb, row_a, row_b, to, steps, ra, rb, tid };
-		Slice f0, f1;
-
 		clear();
 		if (from >= to)
 			return;		/* an empty slice of the axis; the same in every lane of the workgroup */
-		{
-			A a;
-			B b;
-
-			a.start(sa, row_a, from, steps, a0, tid);
-			b.start(sb, row_b, from, steps, b0, tid);
-			a.finish(a0, tid);
-			b.finish(b0, tid);
-			arrived();
-		}
+		a.init(sa, tid);
+		b.init(sb, tid);
+		a.start(sa, row_a, from, steps, lds, tid);
+		b.start(sb, row_b, from, steps, lds + A::kBytes, tid);
+		a.finish(lds, tid);
+		b.finish(lds + A::kBytes, tid);
+		arrived();
 		__syncthreads();
-		read(f0, a0, b0, ra, rb, 0, tid & 63);
-		for (int s = from; s < to; s += 2) {
-			step(w, s, a0, b0, a1, b1, f0, f1);
-			if (s + 1 < to)
-				step(w, s + 1, a1, b1, a0, b0, f0, f1);
+		reada.init(lds, ra, lane);
+		readb.init(lds + A::kBytes, rb, lane);
+		read(f0, reada, readb, 0);
+#pragma unroll 1
+		for (int s = from; s < to; s++) {
+			const bool more = s + 1 < to;
+
+			if (more) {
+				a.start(sa, row_a, s + 1, steps, lds + next, tid);
+				b.start(sb, row_b, s + 1, steps, lds + next + A::kBytes, tid);
+			}
+			read(f1, reada, readb, 1);
+			multiply(f0, sums);
+			__builtin_amdgcn_sched_barrier(0);
+			read(f0, reada, readb, 2);
+			multiply(f1, sums);
+			__builtin_amdgcn_sched_barrier(0);
+			read(f1, reada, readb, 3);
+			multiply(f0, sums);
+			__builtin_amdgcn_sched_barrier(0);
+			if (more) {
+				a.finish(lds + next, tid);
+				b.finish(lds + next + A::kBytes, tid);
+				arrived();
+			}
+			__syncthreads();
+			reada.move(next ? kBuffer : -kBuffer);
+			readb.move(next ? kBuffer : -kBuffer);
+			next = kBuffer - next;
+			/* behind the last step this reads what lies in LDS, for nothing */
+			read(f0, reada, readb, 0);
+			multiply(f1, sums);
+			__builtin_amdgcn_sched_barrier(0);
 		}
+		/* those reads are over before a caller's stores */
+		__syncthreads();
 	}
 };
 
@@ -347,7 +398,8 @@ struct RowArgs {
 	int		d, d_pad, vocab;
 	int64_t		vocab_pad;
 	const float	*bias;		/* may be NULL */
-	uint16_t	*xs;
+	uint16_t	*xs;		/* [rows_pad][ld_xs] */
+	int64_t		ld_xs;
 	int32_t		*ts;
 	float		*bs;
 };
@@ -379,7 +431,7 @@ __global__ __launch_bounds__(kThreads) void head_rows_kernel(RowArgs a)
 					e[j / 2] |= (uint32_t)a.x[r * a.ld_x + c + j] << (16 * (j & 1));
 			w = u32x4{e[0], e[1], e[2], e[3]};
 		}
-		*(u32x4 *)(a.xs + r * a.d_pad + c) = w;
+		*(u32x4 *)(a.xs + r * a.ld_xs + c) = w;
 		if (c == 0)
 			a.ts[r] = live ? t : -1;
 	}
@@ -412,30 +464,20 @@ struct LogitArgs {
 
 enum { kStats = 0, kDelta = 1, kDeltaPair = 2 };
 
-/*
-** Wavefronts of a workgroup for tiles of TT tokens, and how they share the tile: kWavesM along the
-** product's first axis.
-*/
-template <int TT> struct Shape {
-	static constexpr int threads = TT == 256 ? HEAD_T256 : 512;
-	static constexpr int waves = threads / 64;
-};
-
 template <int TT, int MODE>
-__global__ __launch_bounds__(Shape<TT>::threads) void head_logits_kernel(LogitArgs a)
+__global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
 {
-	constexpr int kHeadThreads = Shape<TT>::threads;
-	constexpr int WM = TT == 256 ? 2 : TT == 128 ? 4 : 8, WN = Shape<TT>::waves / WM;
-	typedef Operand<true, true, kSide, kHeadThreads> W;
-	typedef Operand<false, false, TT, kHeadThreads> X;
+	constexpr int WM = TT == 256 ? 2 : TT == 128 ? 4 : 8, WN = kHeadWaves / WM;
+	typedef Operand<true, true, kSide> W;
+	typedef Operand<false, false, TT> X;
 	constexpr int MB = kSide / WM / 32, NB = TT / WN / 32;
-	__shared__ __align__(16) char lw0[W::kBytes], lx0[X::kBytes], lw1[W::kBytes], lx1[X::kBytes];
+	__shared__ __align__(16) char lds[2 * (W::kBytes + X::kBytes)];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	int64_t tv, tt;
-	Product<W, X, MB, NB> prod;
+	Product<W, X, MB, NB, false> prod;
 	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_t, &tv, &tt))
@@ -444,7 +486,7 @@ __global__ __launch_bounds__(Shape<TT>::threads) void head_logits_kernel(LogitAr
 	const int64_t t_tile = tt * TT;
 	const int64_t v_base = v_tile + wm * (MB * 32);
 
-	prod.run(a.w, a.x, v_tile, t_tile, 0, a.steps, a.steps, lw0, lx0, lw1, lx1, wm * (MB * 32), wn * (NB * 32), tid);
+	prod.run(a.w, a.x, v_tile, t_tile, 0, a.steps, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, false);
 #pragma unroll
 	for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -460,12 +502,13 @@ __global__ __launch_bounds__(Shape<TT>::threads) void head_logits_kernel(LogitAr
 				__builtin_amdgcn_sched_barrier(0);	/* all loads ahead of all sums take registers that there are not */
 		}
 	if constexpr (MODE == kStats) {
-		f32x2 *red = (f32x2 *)lw0;	/* [WM][TT]; every wavefront's last read lies before the last step's barrier */
+		f32x2 *red = (f32x2 *)lds;	/* [WM][TT] */
 
 #pragma unroll
 		for (int j = 0; j < NB; j++) {
 			const int t = wn * (NB * 32) + j * 32 + (lane & 31);
-			const int64_t want = (int64_t)a.target[t_tile + t] - v_base;
+			/* the target's place among the lane's rows: a constant for each register */
+			const int want = a.target[t_tile + t] - (int)v_base - block_row(0, lane);
 			float top = -INFINITY, sum = 0.0f, hit = 0.0f;
 
 #pragma unroll
@@ -473,7 +516,7 @@ __global__ __launch_bounds__(Shape<TT>::threads) void head_logits_kernel(LogitAr
 #pragma unroll
 				for (int r = 0; r < 16; r++) {
 					top = fmaxf(top, acc[i][j][r]);
-					if (want == i * 32 + block_row(r, lane))
+					if (want == i * 32 + block_row(r, 0))
 						hit = acc[i][j][r];
 				}
 			top = fmaxf(top, __shfl_xor(top, 32, 64));
@@ -488,7 +531,7 @@ __global__ __launch_bounds__(Shape<TT>::threads) void head_logits_kernel(LogitAr
 			sum += __shfl_xor(sum, 32, 64);
 			if (lane < 32)
 				red[wm * TT + t] = f32x2{top, sum};
-			if (want >= 0 && want < MB * 32 && (int)((want >> 2) & 1) == (lane >> 5))
+			if (want >= 0 && want < MB * 32 && (want & 4) == 0)
 				a.target_logit[t_tile + t] = hit;
 		}
 		__syncthreads();
@@ -509,41 +552,62 @@ __global__ __launch_bounds__(Shape<TT>::threads) void head_logits_kernel(LogitAr
 #pragma unroll
 		for (int j = 0; j < NB; j++) {
 			const int64_t t = t_tile + wn * (NB * 32) + j * 32 + (lane & 31);
-			const int64_t want = (int64_t)a.target[t] - v_base;
+			const int want = a.target[t] - (int)v_base - block_row(0, lane);
 			const bool live = a.target[t] >= 0;
 			const float lse = a.lse[t];
 
 #pragma unroll
 			for (int i = 0; i < MB; i++)
 #pragma unroll
-				for (int q = 0; q < 4; q++) {
-					const int row = i * 32 + block_row(4 * q, lane);
-					const int64_t at = t * a.ld_delta + (v_base - a.v0) + row;
-					float e[4], low[4];
-					u32x2 w;
+				for (int r = 0; r < 16; r++) {
+					float p = __expf(acc[i][j][r] - lse);
+
+					if (want == i * 32 + block_row(r, 0))
+						p -= 1.0f;
+					acc[i][j][r] = live ? p * a.scale : 0.0f;
+				}
+		}
+		/*
+		** A lane holds four places of one token at a time; the tile goes through LDS so that memory is
+		** written in whole lines of 512 bytes (straight from the registers: 16 of every line at a time,
+		** 0.35 ms slower for 4096 tokens of the 555M head).  Chunks are rotated by the token.
+		*/
+#pragma unroll
+		for (int part = 0; part < (MODE == kDeltaPair ? 2 : 1); part++) {
+			uint16_t *out = part ? a.delta_low : a.delta;
 
 #pragma unroll
-					for (int k = 0; k < 4; k++) {
-						float p = __expf(acc[i][j][4 * q + k] - lse);
+			for (int j = 0; j < NB; j++)
+#pragma unroll
+				for (int i = 0; i < MB; i++)
+#pragma unroll
+					for (int q = 0; q < 4; q++) {
+						const int t = wn * (NB * 32) + j * 32 + (lane & 31);
+						const int row = wm * (MB * 32) + i * 32 + block_row(4 * q, lane);
+						u32x2 w;
 
-						if (want == row + k)
-							p -= 1.0f;
-						e[k] = live ? p * a.scale : 0.0f;
+						w.x = bf16_rne2(acc[i][j][4 * q], acc[i][j][4 * q + 1]);
+						w.y = bf16_rne2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+						*(u32x2 *)(lds + t * (kSide * 2) + ((row >> 3) ^ (t & 31)) * 16 + (row & 4) * 2) = w;
+						if constexpr (MODE == kDeltaPair) {
+							/* what the rounding left over, for the second part */
+							acc[i][j][4 * q] -= __uint_as_float(w.x << 16);
+							acc[i][j][4 * q + 1] -= __uint_as_float(w.x & 0xffff0000u);
+							acc[i][j][4 * q + 2] -= __uint_as_float(w.y << 16);
+							acc[i][j][4 * q + 3] -= __uint_as_float(w.y & 0xffff0000u);
+						}
 					}
-					w.x = bf16_rne2(e[0], e[1]);
-					w.y = bf16_rne2(e[2], e[3]);
-					*(u32x2 *)(a.delta + at) = w;
-					if constexpr (MODE == kDeltaPair) {
-						/* what the rounding left over, rounded itself */
-						low[0] = e[0] - __uint_as_float(w.x << 16);
-						low[1] = e[1] - __uint_as_float(w.x & 0xffff0000u);
-						low[2] = e[2] - __uint_as_float(w.y << 16);
-						low[3] = e[3] - __uint_as_float(w.y & 0xffff0000u);
-						w.x = bf16_rne2(low[0], low[1]);
-						w.y = bf16_rne2(low[2], low[3]);
-						*(u32x2 *)(a.delta_low + at) = w;
-					}
-				}
+			__syncthreads();
+#pragma unroll
+			for (int c = tid; c < TT * (kSide / 8); c += kHeadThreads) {
+				const int t = c / (kSide / 8);
+				const int chunk = c % (kSide / 8);
+
+				*(u32x4 *)(out + (t_tile + t) * a.ld_delta + (v_tile - a.v0) + chunk * 8) =
+				    *(const u32x4 *)(lds + t * (kSide * 2) + (chunk ^ (t & 31)) * 16);
+			}
+			if (part == 0 && MODE == kDeltaPair)
+				__syncthreads();
 		}
 	}
 }
@@ -614,14 +678,13 @@ struct DxArgs {
 
 /* One slice of the contracted axis (the vocabulary) per blockIdx.y, each with a slot of its own. */
 template <int TT>
-__global__ __launch_bounds__(Shape<TT>::threads) void head_dx_kernel(DxArgs a)
+__global__ __launch_bounds__(kHeadThreads) void head_dx_kernel(DxArgs a)
 {
-	constexpr int kHeadThreads = Shape<TT>::threads;
-	constexpr int WM = 2, WN = Shape<TT>::waves / WM;
-	typedef Operand<false, false, TT, kHeadThreads> D;
-	typedef Operand<false, true, kSide, kHeadThreads> W;
+	constexpr int WM = 2, WN = kHeadWaves / WM;
+	typedef Operand<false, false, TT> D;
+	typedef Operand<false, true, kSide> W;
 	constexpr int MB = TT / WM / 32, NB = kSide / WN / 32;
-	__shared__ __align__(16) char ld0[D::kBytes], lw0[W::kBytes], ld1[D::kBytes], lw1[W::kBytes];
+	__shared__ __align__(16) char lds[2 * (D::kBytes + W::kBytes)];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -630,13 +693,12 @@ __global__ __launch_bounds__(Shape<TT>::threads) void head_dx_kernel(DxArgs a)
 	const int from = (int)((int64_t)total * blockIdx.y / a.splits);
 	const int to = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
 	int64_t tt, td;
-	Product<D, W, MB, NB> prod;
+	Product<D, W, MB, NB, false> prod;
 	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_t, a.tiles_d, &tt, &td))
 		return;
-	prod.run(a.delta, a.w, tt * TT, td * kSide, from, to, a.steps, ld0, lw0, ld1, lw1, wm * (MB * 32), wn * (NB * 32),
-	    tid);
+	prod.run(a.delta, a.w, tt * TT, td * kSide, from, to, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, false);
 #pragma unroll
 	for (int i = 0; i < MB; i++)
 #pragma unroll
@@ -696,10 +758,11 @@ struct DwArgs {
 	int64_t		tiles_d, tiles_v;
 	int		d, vocab;
 	int64_t		v0;
-	void		*dw;		/* [d][vocab] */
+	void		*dw;		/* [d][vocab] or NULL */
 	void		*db;		/* [vocab] or NULL */
 };
 
+/* base[i] += x */
 template <int GT>
 __device__ __forceinline__ void add_to(void *base, int64_t i, float x)
 {
@@ -710,76 +773,117 @@ __device__ __forceinline__ void add_to(void *base, int64_t i, float x)
 }
 
 template <int GT>
-__global__ __launch_bounds__(Shape<256>::threads) void head_dw_kernel(DwArgs a)
+__global__ __launch_bounds__(kHeadThreads) void head_dw_kernel(DwArgs a)
 {
-	constexpr int kHeadThreads = Shape<256>::threads;
-	constexpr int WM = 2, WN = Shape<256>::waves / WM;
-	typedef Operand<true, false, kSide, kHeadThreads> X;
-	typedef Operand<true, false, kSide, kHeadThreads> D;
+	constexpr int WM = 2, WN = kHeadWaves / WM;
+	typedef Operand<true, false, kSide> X;
+	typedef Operand<true, false, kSide> D;
 	constexpr int MB = kSide / WM / 32, NB = kSide / WN / 32;
-	__shared__ __align__(16) char lx0[X::kBytes], ld0[D::kBytes], lx1[X::kBytes], ld1[D::kBytes];
+	__shared__ __align__(16) char lds[2 * (X::kBytes + D::kBytes)];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	int64_t td, tv;
-	Product<X, D, MB, NB> prod;
+	Product<X, D, MB, NB, true> prod;
 	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_d, &tv, &td))
 		return;
-	prod.run(a.x, a.delta, td * kSide, tv * kSide, 0, a.steps * a.parts, a.steps, lx0, ld0, lx1, ld1, wm * (MB * 32),
-	    wn * (NB * 32), tid);
-#pragma unroll
-	for (int j = 0; j < NB; j++) {
-		const int64_t v = a.v0 + tv * kSide + wn * (NB * 32) + j * 32 + (lane & 31);
+	/* the column sums: in the tiles of the first rows of x^T, by the wavefronts that hold the upper half */
+	const bool sums = a.db != nullptr && td == 0 && wm == 0;
 
-		if (v >= a.vocab)
-			continue;
+	prod.run(a.x, a.delta, td * kSide, tv * kSide, 0, a.steps * a.parts, a.steps, lds, wm * (MB * 32),
+	    wn * (NB * 32), tid, sums);
+	if (sums && lane < 32) {
 #pragma unroll
-		for (int i = 0; i < MB; i++)
-#pragma unroll
-			for (int r = 0; r < 16; r++) {
-				const int64_t c = td * kSide + wm * (MB * 32) + i * 32 + block_row(r, lane);
+		for (int j = 0; j < NB; j++) {
+			const int64_t v = a.v0 + tv * kSide + wn * (NB * 32) + j * 32 + lane;
 
-				if (c < a.d)
-					add_to<GT>(a.dw, c * a.vocab + v, acc[i][j][r]);
-			}
+			if (v < a.vocab)
+				add_to<GT>(a.db, v, prod.sum[j][0]);
+		}
 	}
-}
+	if (!a.dw)
+		return;
+	/*
+	** The tile through LDS, half its rows at a time, so that dw is read and written in whole lines (a
+	** lane holds one column: two bytes of a line with bf16 gradients, and 96 tokens of the 555M head,
+	** where this is most of the work, took 620 us).
+	*/
+	constexpr int kWide = GT == kF32 ? 4 : 8;		/* elements in sixteen bytes */
+	constexpr int kHalf = kSide / 2;
+	constexpr int kAhead = 8;
+	float *const tile = (float *)lds;			/* [kHalf][kSide] */
 
-struct DbArgs {
-	const uint16_t	*delta[2];
-	int		parts;
-	int64_t		ld, rows_pad;
-	int64_t		v0;
-	int		count;		/* columns of this piece */
-	void		*db;
-};
+#pragma unroll
+	for (int h = 0; h < 2; h++) {
+		if (h)
+			__syncthreads();
+#pragma unroll
+		for (int i = 0; i < MB / 2; i++)
+#pragma unroll
+			for (int j = 0; j < NB; j++)
+#pragma unroll
+				for (int r = 0; r < 16; r++)
+					tile[(wm * (kHalf / 2) + i * 32 + block_row(r, lane)) * kSide + wn * (NB * 32) + j * 32
+					    + (lane & 31)] = acc[h * (MB / 2) + i][j][r];
+		__syncthreads();
+		for (int c0 = tid; c0 < kHalf * kSide / kWide; c0 += kAhead * kHeadThreads) {
+			u32x4 old[kAhead];
 
-/* db += column sums of delta: 64 columns to a workgroup, rows shared by its wavefronts, fixed order. */
-template <int GT>
-__global__ __launch_bounds__(512) void head_db_kernel(DbArgs a)
-{
-	__shared__ float red[8][64];
-	const int lane = threadIdx.x & 63;
-	const int wave = threadIdx.x >> 6;
-	const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-	float s = 0.0f;
+#pragma unroll
+			for (int u = 0; u < kAhead; u++) {
+				const int c = c0 + u * kHeadThreads;
+				const int row = c / (kSide / kWide);
+				const int64_t k = td * kSide + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
+				const int64_t v = a.v0 + tv * kSide + c % (kSide / kWide) * kWide;
 
-	for (int p = 0; p < a.parts; p++)
-		for (int64_t r = wave; r < a.rows_pad; r += 8)
-			s += bf16_widen(a.delta[p][r * a.ld + c]);
-	red[wave][lane] = s;
-	__syncthreads();
-	if (wave == 0 && c < a.count) {
-		for (int k = 1; k < 8; k++)
-			s += red[k][lane];
-		add_to<GT>(a.db, a.v0 + c, s);
+				if (k < a.d && v + kWide <= a.vocab)
+					old[u] = *(const u32x4_any *)((const char *)a.dw + (k * a.vocab + v) * (16 / kWide));
+			}
+#pragma unroll
+			for (int u = 0; u < kAhead; u++) {
+				const int c = c0 + u * kHeadThreads;
+				const int row = c / (kSide / kWide);
+				const int64_t k = td * kSide + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
+				const int64_t v = a.v0 + tv * kSide + c % (kSide / kWide) * kWide;
+				const float *x = tile + row * kSide + c % (kSide / kWide) * kWide;
+
+				if (k >= a.d)
+					continue;
+				if (v + kWide <= a.vocab) {
+					u32x4 w;
+
+					if constexpr (GT == kF32) {
+#pragma unroll
+						for (int e = 0; e < 4; e++)
+							w[e] = __float_as_uint(__uint_as_float(old[u][e]) + x[e]);
+					} else {
+#pragma unroll
+						for (int e = 0; e < 4; e++)
+							w[e] = bf16_rne2(__uint_as_float(old[u][e] << 16) + x[2 * e],
+							    __uint_as_float(old[u][e] & 0xffff0000u) + x[2 * e + 1]);
+					}
+					*(u32x4_any *)((char *)a.dw + (k * a.vocab + v) * (16 / kWide)) = w;
+				} else {
+					for (int e = 0; e < kWide; e++)
+						if (v + e < a.vocab)
+							add_to<GT>(a.dw, k * a.vocab + v + e, x[e]);
+				}
+			}
+		}
 	}
 }
 
 /* ---- plan -------------------------------------------------------------------------------------- */
+
+/*
+** The work area's matrices have lines of an odd number of 256 bytes.  Lines of a power of two put a
+** tile's column of lines into one of the sixteen channels of the level-two cache.
+*/
+constexpr int kOdd = 128;
+static_assert((kSide + kOdd) * 2 % 512 == 256, "lines of whole tiles, then 256 bytes");
 
 struct HeadPlan {
 	int	tile_t;		/* tokens per tile */
@@ -787,6 +891,7 @@ struct HeadPlan {
 	int	d_pad;
 	int64_t	tiles_v;	/* of the whole vocabulary */
 	int64_t	piece;		/* vocabulary places per piece of delta, a multiple of kSide */
+	int64_t	ld_xs, ld_delta;
 	int	parts;		/* bf16 numbers per element of delta */
 	int	splits;		/* slices of the vocabulary in dx */
 	size_t	off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_slot;
@@ -817,8 +922,9 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	p->d_pad = (int)up((size_t)d, kSide);
 	p->tiles_v = (vocab + kSide - 1) / kSide;
 	p->parts = grad_type == ANNI_F32 ? 2 : 1;
+	p->ld_xs = p->d_pad + kOdd;
 	p->off_xs = at;
-	at = up(at + (size_t)p->rows_pad * p->d_pad * 2, 256);
+	at = up(at + (size_t)p->rows_pad * p->ld_xs * 2, 256);
 	p->off_ts = at;
 	at = up(at + (size_t)p->rows_pad * 4, 256);
 	p->off_bs = at;
@@ -836,12 +942,13 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		int64_t steps;
 
 		p->piece = whole <= fit ? whole : fit < kSide ? kSide : fit;
+		p->ld_delta = p->piece + kOdd;
 		steps = p->piece / kStep * p->parts;
 		p->splits = 1;
 		while (tiles * p->splits < 512 && steps / (p->splits * 2) >= 8)
 			p->splits *= 2;
 		p->off_delta = at;
-		at = up(at + (size_t)p->rows_pad * p->piece * 2 * p->parts, 256);
+		at = up(at + (size_t)p->rows_pad * p->ld_delta * 2 * p->parts, 256);
 		p->off_slot = at;
 		at = up(at + (size_t)p->splits * p->rows_pad * p->d_pad * 4, 256);
 	}
@@ -862,11 +969,11 @@ static void logits_launch(hipStream_t st, int tile_t, const LogitArgs &a)
 	const dim3 grid((unsigned)up((size_t)(a.tiles_v * a.tiles_t), 8));
 
 	if (tile_t == 64)
-		hipLaunchKernelGGL((head_logits_kernel<64, MODE>), grid, dim3(Shape<64>::threads), 0, st, a);
+		hipLaunchKernelGGL((head_logits_kernel<64, MODE>), grid, dim3(kHeadThreads), 0, st, a);
 	else if (tile_t == 128)
-		hipLaunchKernelGGL((head_logits_kernel<128, MODE>), grid, dim3(Shape<128>::threads), 0, st, a);
+		hipLaunchKernelGGL((head_logits_kernel<128, MODE>), grid, dim3(kHeadThreads), 0, st, a);
 	else
-		hipLaunchKernelGGL((head_logits_kernel<256, MODE>), grid, dim3(Shape<256>::threads), 0, st, a);
+		hipLaunchKernelGGL((head_logits_kernel<256, MODE>), grid, dim3(kHeadThreads), 0, st, a);
 }
 
 static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
@@ -893,6 +1000,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	ra.vocab_pad = p.tiles_v * kSide;
 	ra.bias = j.d_bias;
 	ra.xs = xs;
+	ra.ld_xs = p.ld_xs;
 	ra.ts = ts;
 	ra.bs = (float *)(work + p.off_bs);
 	hipLaunchKernelGGL(head_rows_kernel, dim3(rows_grid(p.rows_pad * (p.d_pad / 8))), dim3(kThreads), 0, st, ra);
@@ -904,7 +1012,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	la.w.depth = j.d;
 	la.w.aligned = ((uintptr_t)w & 15) == 0 && j.vocab % 8 == 0;
 	la.x.part[0] = la.x.part[1] = xs;
-	la.x.ld = (uint32_t)p.d_pad;
+	la.x.ld = (uint32_t)p.ld_xs;
 	la.x.rows = p.rows_pad;
 	la.x.depth = p.d_pad;
 	la.bias = ra.bs;
@@ -932,7 +1040,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		const int64_t left = j.vocab - v0;
 		const int64_t here = left < p.piece ? (int64_t)up((size_t)left, kSide) : p.piece;
 		uint16_t *delta = (uint16_t *)(work + p.off_delta);
-		uint16_t *low = delta + p.rows_pad * p.piece;
+		uint16_t *low = delta + p.rows_pad * p.ld_delta;
 		DxArgs xa;
 		DwArgs wa;
 
@@ -942,7 +1050,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		la.scale = (float)j.scale;
 		la.delta = delta;
 		la.delta_low = low;
-		la.ld_delta = p.piece;
+		la.ld_delta = p.ld_delta;
 		if (p.parts == 2)
 			logits_launch<kDeltaPair>(st, p.tile_t, la);
 		else
@@ -954,7 +1062,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		wa.x.depth = p.rows_pad;
 		wa.delta.part[0] = delta;
 		wa.delta.part[1] = low;
-		wa.delta.ld = (uint32_t)p.piece;
+		wa.delta.ld = (uint32_t)p.ld_delta;
 		wa.delta.rows = here;
 		wa.delta.depth = p.rows_pad;
 		wa.steps = (int)(p.rows_pad / kStep);
@@ -966,30 +1074,15 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		wa.v0 = v0;
 		wa.dw = j.d_dw;
 		wa.db = j.d_db;
+		if (!j.d_dw)
+			wa.tiles_d = 1;			/* only the tiles that sum */
 		const dim3 wgrid((unsigned)up((size_t)(wa.tiles_d * wa.tiles_v), 8));
 
-		if (j.d_dw) {
+		if (j.d_dw || j.d_db) {
 			if (j.grad_type == ANNI_F32)
-				hipLaunchKernelGGL(head_dw_kernel<kF32>, wgrid, dim3(Shape<256>::threads), 0, st, wa);
+				hipLaunchKernelGGL(head_dw_kernel<kF32>, wgrid, dim3(kHeadThreads), 0, st, wa);
 			else
-				hipLaunchKernelGGL(head_dw_kernel<kBF16>, wgrid, dim3(Shape<256>::threads), 0, st, wa);
-		}
-		if (j.d_db) {
-			DbArgs ba;
-
-			memset(&ba, 0, sizeof(ba));
-			ba.delta[0] = delta;
-			ba.delta[1] = low;
-			ba.parts = p.parts;
-			ba.ld = p.piece;
-			ba.rows_pad = p.rows_pad;
-			ba.v0 = v0;
-			ba.count = (int)(left < here ? left : here);
-			ba.db = j.d_db;
-			if (j.grad_type == ANNI_F32)
-				hipLaunchKernelGGL(head_db_kernel<kF32>, dim3((unsigned)(here / 64)), dim3(512), 0, st, ba);
-			else
-				hipLaunchKernelGGL(head_db_kernel<kBF16>, dim3((unsigned)(here / 64)), dim3(512), 0, st, ba);
+				hipLaunchKernelGGL(head_dw_kernel<kBF16>, wgrid, dim3(kHeadThreads), 0, st, wa);
 		}
 		if (j.d_dx) {
 			memset(&xa, 0, sizeof(xa));
@@ -1013,11 +1106,11 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			const dim3 grid((unsigned)up((size_t)(xa.tiles_t * xa.tiles_d), 8), (unsigned)p.splits);
 
 			if (p.tile_t == 64)
-				hipLaunchKernelGGL(head_dx_kernel<64>, grid, dim3(Shape<64>::threads), 0, st, xa);
+				hipLaunchKernelGGL(head_dx_kernel<64>, grid, dim3(kHeadThreads), 0, st, xa);
 			else if (p.tile_t == 128)
-				hipLaunchKernelGGL(head_dx_kernel<128>, grid, dim3(Shape<128>::threads), 0, st, xa);
+				hipLaunchKernelGGL(head_dx_kernel<128>, grid, dim3(kHeadThreads), 0, st, xa);
 			else
-				hipLaunchKernelGGL(head_dx_kernel<256>, grid, dim3(Shape<256>::threads), 0, st, xa);
+				hipLaunchKernelGGL(head_dx_kernel<256>, grid, dim3(kHeadThreads), 0, st, xa);
 		}
 	}
 	if (grad && j.d_dx) {
