@@ -102,12 +102,13 @@ struct Operand {
 
 	static __device__ __forceinline__ int turn(int line)
 	{
-		return BY_ROW ? (line & 3) << 2 : line & 7;
+		/* sixteen lanes of a read at a time: by row four lines of two chunks, else sixteen lines of one */
+		return BY_ROW ? (line & 3) << 2 : (line >> 1) & 7;
 	}
 
 	__device__ __forceinline__ void init(const Source &src, int tid)
 	{
-		static_assert(kApart % 8 == 0, "turn() is the same for all chunks of a lane");
+		static_assert(kApart % (BY_ROW ? 4 : 16) == 0, "turn() is the same for all chunks of a lane");
 		line = tid / kLine;
 		col = ((tid % kLine) ^ turn(line)) * 8;
 		offset = (uint32_t)line * src.ld + (uint32_t)col;
@@ -306,7 +307,7 @@ struct Product {
 		ReadA reada;
 		ReadB readb;
 		Slice f0, f1;
-		int next = kBuffer;		/* where the half for the next step begins */
+		int here = 0;			/* where the half that is computed on begins */
 
 		static_assert(kStep == 64, "four slices");
 		clear();
@@ -320,17 +321,17 @@ struct Product {
 		b.finish(lds + A::kBytes, tid);
 		arrived();
 		__syncthreads();
+		if (from + 1 < to) {
+			a.start(sa, row_a, from + 1, steps, lds + kBuffer, tid);
+			b.start(sb, row_b, from + 1, steps, lds + kBuffer + A::kBytes, tid);
+		}
 		reada.init(lds, ra, lane);
 		readb.init(lds + A::kBytes, rb, lane);
 		read(f0, reada, readb, 0);
 #pragma unroll 1
 		for (int s = from; s < to; s++) {
-			const bool more = s + 1 < to;
+			const int other = kBuffer - here;
 
-			if (more) {
-				a.start(sa, row_a, s + 1, steps, lds + next, tid);
-				b.start(sb, row_b, s + 1, steps, lds + next + A::kBytes, tid);
-			}
 			read(f1, reada, readb, 1);
 			multiply(f0, sums);
 			__builtin_amdgcn_sched_barrier(0);
@@ -340,15 +341,20 @@ struct Product {
 			read(f1, reada, readb, 3);
 			multiply(f0, sums);
 			__builtin_amdgcn_sched_barrier(0);
-			if (more) {
-				a.finish(lds + next, tid);
-				b.finish(lds + next + A::kBytes, tid);
+			if (s + 1 < to) {
+				a.finish(lds + other, tid);
+				b.finish(lds + other + A::kBytes, tid);
 				arrived();
 			}
 			__syncthreads();
-			reada.move(next ? kBuffer : -kBuffer);
-			readb.move(next ? kBuffer : -kBuffer);
-			next = kBuffer - next;
+			if (s + 2 < to) {
+				/* ahead of the products: issuing those takes the wavefront as long as they run */
+				a.start(sa, row_a, s + 2, steps, lds + here, tid);
+				b.start(sb, row_b, s + 2, steps, lds + here + A::kBytes, tid);
+			}
+			reada.move(other - here);
+			readb.move(other - here);
+			here = other;
 			/* behind the last step this reads what lies in LDS, for nothing */
 			read(f0, reada, readb, 0);
 			multiply(f1, sums);
