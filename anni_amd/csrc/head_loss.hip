@@ -139,15 +139,22 @@ struct Operand {
 			const int cols = (int)(BY_ROW ? (rows_left < ROWS ? rows_left : ROWS)
 			    : (depth_left < kStep ? depth_left : kStep));
 
+			/* a lane's chunks share their place in the line: all of them whole, or none */
+			if (col + 8 <= cols) {
 #pragma unroll
-			for (int i = 0; i < kChunks; i++) {
-				const int at = line + i * kApart;
-				const uint16_t *q = base + (uint32_t)(at < lines ? at : lines - 1) * src.ld + (uint32_t)col;
-				u32x4 w = {0u, 0u, 0u, 0u};
+				for (int i = 0; i < kChunks; i++) {
+					const int at = line + i * kApart;
 
-				if (col + 8 <= cols) {
-					w = *(const u32x4_any *)q;
-				} else {
+					hold[i] = *(const u32x4_any *)(base + (uint32_t)(at < lines ? at : lines - 1) * src.ld
+					    + (uint32_t)col);
+				}
+			} else {
+#pragma unroll
+				for (int i = 0; i < kChunks; i++) {
+					const int at = line + i * kApart;
+					const uint16_t *q = base + (uint32_t)(at < lines ? at : lines - 1) * src.ld + (uint32_t)col;
+					u32x4 w = {0u, 0u, 0u, 0u};
+
 					/* from the last element down, each pushing the others up */
 #pragma unroll 1
 					for (int j = 7; j >= 0; j--) {
@@ -158,8 +165,8 @@ struct Operand {
 						w.y = (w.y << 16) | (w.x >> 16);
 						w.x = (w.x << 16) | e;
 					}
+					hold[i] = w;
 				}
-				hold[i] = w;
 			}
 		}
 	}
@@ -705,18 +712,28 @@ __global__ __launch_bounds__(kHeadThreads) void head_dx_kernel(DxArgs a)
 	if (!tile_of(blockIdx.x, a.tiles_t, a.tiles_d, &tt, &td))
 		return;
 	prod.run(a.delta, a.w, tt * TT, td * kSide, from, to, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, false);
+	/* a block at a time: its old values are all on their way before the first store */
 #pragma unroll
 	for (int i = 0; i < MB; i++)
 #pragma unroll
-		for (int j = 0; j < NB; j++)
-#pragma unroll
-			for (int r = 0; r < 16; r++) {
-				const int64_t t = tt * TT + wm * (MB * 32) + i * 32 + block_row(r, lane);
-				const int64_t c = td * kSide + wn * (NB * 32) + j * 32 + (lane & 31);
-				float *p = a.slot + ((int64_t)blockIdx.y * a.rows_pad + t) * a.d_pad + c;
+		for (int j = 0; j < NB; j++) {
+			const int64_t t = tt * TT + wm * (MB * 32) + i * 32 + block_row(0, lane);
+			const int64_t c = td * kSide + wn * (NB * 32) + j * 32 + (lane & 31);
+			float *p = a.slot + ((int64_t)blockIdx.y * a.rows_pad + t) * a.d_pad + c;
+			float old[16];
 
-				*p = a.add ? *p + acc[i][j][r] : acc[i][j][r];
+			if (a.add) {
+#pragma unroll
+				for (int r = 0; r < 16; r++)
+					old[r] = p[(int64_t)block_row(r, 0) * a.d_pad];
+#pragma unroll
+				for (int r = 0; r < 16; r++)
+					acc[i][j][r] += old[r];
 			}
+#pragma unroll
+			for (int r = 0; r < 16; r++)
+				p[(int64_t)block_row(r, 0) * a.d_pad] = acc[i][j][r];
+		}
 }
 
 struct DxSumArgs {
@@ -742,6 +759,7 @@ __global__ __launch_bounds__(kThreads) void head_dx_sum_kernel(DxSumArgs a)
 
 		if (c >= a.d)
 			continue;
+#pragma unroll 8
 		for (int k = 0; k < a.splits; k++)
 			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_pad + c);
 #pragma unroll
@@ -909,6 +927,7 @@ static size_t up(size_t x, size_t a)
 	return (x + a - 1) / a * a;
 }
 
+static const int kUnits = 256;		/* compute units of an MI355X, a workgroup of a large tile each */
 static const int64_t kHeadMaxRows = (int64_t)1 << 22;
 static const int kHeadMaxD = 1 << 16;
 static const int kHeadMaxVocab = 1 << 22;
@@ -947,12 +966,25 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		const int64_t tiles = p->rows_pad / p->tile_t * (p->d_pad / kSide);
 		int64_t steps;
 
-		p->piece = whole <= fit ? whole : fit < kSide ? kSide : fit;
+		const int64_t pieces = fit < kSide ? whole / kSide : (whole + fit - 1) / fit;
+
+		/* pieces of about the same size: the last one would leave compute units idle */
+		p->piece = (int64_t)up((size_t)((whole + pieces - 1) / pieces), kSide);
 		p->ld_delta = p->piece + kOdd;
 		steps = p->piece / kStep * p->parts;
+		/*
+		** Slices of the vocabulary in dx, each with a float slot for the whole of dx: the fewest that fill
+		** nine tenths of the compute units' turns, of at least sixteen steps each.
+		*/
 		p->splits = 1;
-		while (tiles * p->splits < 512 && steps / (p->splits * 2) >= 8)
-			p->splits *= 2;
+		for (int k = 1; k <= 64 && k * 16 <= steps; k++) {
+			const int64_t groups = tiles * k;
+			const int64_t turns = (groups + kUnits - 1) / kUnits;
+
+			p->splits = k;
+			if (groups * 10 >= turns * kUnits * 9)
+				break;
+		}
 		p->off_delta = at;
 		at = up(at + (size_t)p->rows_pad * p->ld_delta * 2 * p->parts, 256);
 		p->off_slot = at;
