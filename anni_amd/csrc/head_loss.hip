@@ -40,8 +40,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 /* sixteen bytes at any element: rows of an odd vocabulary are not aligned (the hardware does not mind) */
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-constexpr int kHeadWaves = 8;		/* two to a SIMD */
-constexpr int kHeadThreads = kHeadWaves * 64;
 constexpr int kStep = 64;		/* of the contracted axis per trip */
 constexpr int kSide = 256;		/* of a result tile along the vocabulary or the model's width */
 
@@ -59,6 +57,7 @@ constexpr int kSide = 256;		/* of a result tile along the vocabulary or the mode
 ** CHECK: the array ends inside tiles or its lines are not aligned to 16 bytes; such tiles go through
 ** registers.  Loads never leave the array: what lies beyond along the contiguous axis reads as 0,
 ** beyond along the other one the last valid line again (its product is with zeros, or not kept).
+** There has to be one: no tile or step is launched whose first line lies beyond the array.
 */
 struct Source {
 	const uint16_t	*part[2];	/* second: the low halves, same shape */
@@ -83,18 +82,20 @@ __device__ __forceinline__ void memory_to_lds(const uint16_t *base, uint32_t off
 	    : : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(base) : "memory");
 }
 
+/* All but the LATER last loads have arrived. */
+template <int LATER>
 __device__ __forceinline__ void arrived(void)
 {
-	asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+	asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LATER) : "memory");
 }
 
 /* One lane's place in an operand: kept across the steps, all else is uniform (registers are what is short). */
-template <bool BY_ROW, bool CHECK, int ROWS>
+template <bool BY_ROW, bool CHECK, int ROWS, int THREADS>
 struct Operand {
-	static constexpr int kChunks = ROWS * kStep / 8 / kHeadThreads;
+	static constexpr int kChunks = ROWS * kStep / 8 / THREADS;
 	static constexpr int kBytes = ROWS * kStep * 2;
 	static constexpr int kLine = BY_ROW ? ROWS / 8 : kStep / 8;	/* chunks to a line */
-	static constexpr int kApart = kHeadThreads / kLine;		/* lines between two chunks of a lane */
+	static constexpr int kApart = THREADS / kLine;		/* lines between two chunks of a lane */
 	uint32_t	offset;		/* elements from the tile's start to the lane's first chunk */
 	int		line, col;	/* its line, and its place in it */
 	u32x4		hold[CHECK ? kChunks : 1];
@@ -102,8 +103,13 @@ struct Operand {
 
 	static __device__ __forceinline__ int turn(int line)
 	{
-		/* sixteen lanes of a read at a time: by row four lines of two chunks, else sixteen lines of one */
-		return BY_ROW ? (line & 3) << 2 : (line >> 1) & 7;
+		/*
+		** LDS serves 256 bytes at a time: sixteen lines of one chunk, or by row 32 lanes with half a chunk
+		** each, four lines of four chunks.  Short lines share those 256 bytes.
+		*/
+		if (!BY_ROW)
+			return (line >> 1) & 7;
+		return kLine == 8 ? (line & 2) << 1 : (line & 3) << 2;
 	}
 
 	__device__ __forceinline__ void init(const Source &src, int tid)
@@ -112,6 +118,12 @@ struct Operand {
 		line = tid / kLine;
 		col = ((tid % kLine) ^ turn(line)) * 8;
 		offset = (uint32_t)line * src.ld + (uint32_t)col;
+	}
+
+	/* Do all of the tile's steps go through registers? */
+	static __device__ __forceinline__ bool always_held(const Source &src, int64_t row0)
+	{
+		return CHECK && (src.rows - row0 < ROWS || !src.aligned);
 	}
 
 	/* Step `s` (of `steps` per part) on its way to `lds`, or into registers. */
@@ -130,7 +142,7 @@ struct Operand {
 #pragma unroll
 			for (int i = 0; i < kChunks; i++)
 				memory_to_lds(base + (int64_t)(i * kApart) * src.ld, offset * 2,
-				    lds + (i * kHeadThreads + wave * 64) * 16);
+				    lds + (i * THREADS + wave * 64) * 16);
 			return;
 		}
 		if constexpr (CHECK) {
@@ -178,7 +190,7 @@ struct Operand {
 			if (held)
 #pragma unroll
 				for (int i = 0; i < kChunks; i++)
-					*(u32x4 *)(lds + (tid + i * kHeadThreads) * 16) = hold[i];
+					*(u32x4 *)(lds + (tid + i * THREADS) * 16) = hold[i];
 		}
 	}
 
@@ -241,16 +253,20 @@ struct Operand {
 /*
 ** acc += A B^T over the steps [from, to): acc[i][j] is the 32 x 32 block (i, j) of the wavefront's part.
 **
-** A step's operands are on their way into one half of LDS while the other half is computed on, and
-** the fragments of a 16-deep slice are read while the slice before is multiplied.  The one barrier
-** of a step stands before its last slice's products, whose fragments are in registers by then: behind
-** it the first fragments of the next step are read under those products, and the half that everyone
-** has read is filled again.
+** LDS holds STAGES steps: one that is computed on, the others on their way.  The fragments of a
+** 16-deep slice are read while the slice before is multiplied.  The one barrier of a step stands
+** before its last slice's products, whose fragments are in registers by then: behind it the first
+** fragments of the next step are read under those products, and the stage that everyone has read is
+** filled again.  Large tiles are bound by the matrix pipes and take two stages; the small ones are
+** bound by memory and need more on its way.
+**
+** Operands that go through registers (`held`) are one step ahead whatever STAGES, or, where that is
+** only the last step of an axis that ends inside it, are put away as soon as they come.
 **
 ** SUMS: on request also sum[j] = the sums of B's rows over the contracted axis (every register of a
 ** lane the same), by products with ones: two more matrix instructions to eight.
 */
-template <class A, class B, int MB, int NB, bool SUMS>
+template <class A, class B, int MB, int NB, int STAGES, bool SUMS>
 struct Product {
 	f32x16	acc[MB][NB];
 	f32x16	sum[SUMS ? NB : 1];
@@ -307,14 +323,18 @@ struct Product {
 	__device__ __forceinline__ void run(const Source &sa, const Source &sb, int64_t row_a, int64_t row_b, int from,
 		int to, int steps, char *lds, int ra, int rb, int tid, bool sums)
 	{
-		constexpr int kBuffer = A::kBytes + B::kBytes;
+		constexpr int kStage = A::kBytes + B::kBytes;
+		constexpr int kLater = (STAGES - 2) * (A::kChunks + B::kChunks);	/* loads of the steps after the next */
 		const int lane = tid & 63;
+		/* steps ahead: all stages, if nothing but an axis' last step goes through registers */
+		const bool deep = STAGES > 2 && !A::always_held(sa, row_a) && !B::always_held(sb, row_b);
+		const int ahead = deep ? STAGES - 1 : 1;
 		A a;
 		B b;
 		ReadA reada;
 		ReadB readb;
 		Slice f0, f1;
-		int here = 0;			/* where the half that is computed on begins */
+		int here = 0;			/* where the stage that is computed on begins */
 
 		static_assert(kStep == 64, "four slices");
 		clear();
@@ -322,22 +342,22 @@ struct Product {
 			return;		/* an empty slice of the axis; the same in every lane of the workgroup */
 		a.init(sa, tid);
 		b.init(sb, tid);
-		a.start(sa, row_a, from, steps, lds, tid);
-		b.start(sb, row_b, from, steps, lds + A::kBytes, tid);
-		a.finish(lds, tid);
-		b.finish(lds + A::kBytes, tid);
-		arrived();
-		__syncthreads();
-		if (from + 1 < to) {
-			a.start(sa, row_a, from + 1, steps, lds + kBuffer, tid);
-			b.start(sb, row_b, from + 1, steps, lds + kBuffer + A::kBytes, tid);
+		for (int k = 0; k < ahead && from + k < to; k++) {
+			a.start(sa, row_a, from + k, steps, lds + k * kStage, tid);
+			b.start(sb, row_b, from + k, steps, lds + k * kStage + A::kBytes, tid);
+			a.finish(lds + k * kStage, tid);
+			b.finish(lds + k * kStage + A::kBytes, tid);
 		}
+		arrived<0>();
+		__syncthreads();
 		reada.init(lds, ra, lane);
 		readb.init(lds + A::kBytes, rb, lane);
+		if (from + ahead < to)
+			begin(a, b, sa, sb, row_a, row_b, from + ahead, steps, lds + ahead * kStage, deep, tid);
 		read(f0, reada, readb, 0);
 #pragma unroll 1
 		for (int s = from; s < to; s++) {
-			const int other = kBuffer - here;
+			const int next = here + kStage < (ahead + 1) * kStage ? here + kStage : 0;
 
 			read(f1, reada, readb, 1);
 			multiply(f0, sums);
@@ -349,19 +369,22 @@ struct Product {
 			multiply(f0, sums);
 			__builtin_amdgcn_sched_barrier(0);
 			if (s + 1 < to) {
-				a.finish(lds + other, tid);
-				b.finish(lds + other + A::kBytes, tid);
-				arrived();
+				if (!deep) {
+					a.finish(lds + next, tid);
+					b.finish(lds + next + A::kBytes, tid);
+				}
+				if (deep && s + ahead < to)
+					arrived<kLater>();
+				else
+					arrived<0>();
 			}
 			__syncthreads();
-			if (s + 2 < to) {
-				/* ahead of the products: issuing those takes the wavefront as long as they run */
-				a.start(sa, row_a, s + 2, steps, lds + here, tid);
-				b.start(sb, row_b, s + 2, steps, lds + here + A::kBytes, tid);
-			}
-			reada.move(other - here);
-			readb.move(other - here);
-			here = other;
+			/* ahead of the products: issuing those takes the wavefront as long as they run */
+			if (s + 1 + ahead < to)
+				begin(a, b, sa, sb, row_a, row_b, s + 1 + ahead, steps, lds + here, deep, tid);
+			reada.move(next - here);
+			readb.move(next - here);
+			here = next;
 			/* behind the last step this reads what lies in LDS, for nothing */
 			read(f0, reada, readb, 0);
 			multiply(f1, sums);
@@ -369,6 +392,17 @@ struct Product {
 		}
 		/* those reads are over before a caller's stores */
 		__syncthreads();
+	}
+
+	static __device__ __forceinline__ void begin(A &a, B &b, const Source &sa, const Source &sb, int64_t row_a,
+		int64_t row_b, int s, int steps, char *lds, bool deep, int tid)
+	{
+		a.start(sa, row_a, s, steps, lds, tid);
+		b.start(sb, row_b, s, steps, lds + A::kBytes, tid);
+		if (deep) {
+			a.finish(lds, tid);
+			b.finish(lds + A::kBytes, tid);
+		}
 	}
 };
 
@@ -477,25 +511,51 @@ struct LogitArgs {
 
 enum { kStats = 0, kDelta = 1, kDeltaPair = 2 };
 
-template <int TT, int MODE>
-__global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
+/* A tile of VOCAB places and TOKENS tokens, or of the model's width and tokens, to a workgroup. */
+template <int SIDE_, int TOKENS_, int WAVES_, int WAVES_SIDE_, int STAGES_> struct Shape {
+	static constexpr int side = SIDE_;
+	static constexpr int tokens = TOKENS_;
+	static constexpr int waves = WAVES_;
+	static constexpr int threads = WAVES_ * 64;
+	static constexpr int waves_side = WAVES_SIDE_;		/* wavefronts along the side */
+	static constexpr int waves_tokens = WAVES_ / WAVES_SIDE_;
+	static constexpr int stages = STAGES_;
+};
+
+/*
+** Few tokens: the products are bound by reading w once.  Small tiles, so that there are workgroups for
+** all compute units and two or three to each, with three stages on their way.  Many tokens: two stages
+** of the largest tile that fits.  In between: half of it along the tokens.
+*/
+typedef Shape<64, 64, 4, 2, 4> LogitsFew;
+typedef Shape<64, 128, 4, 2, 3> LogitsSome;
+typedef Shape<256, 128, 8, 4, 3> LogitsMore;
+typedef Shape<256, 256, 8, 2, 2> LogitsMany;
+typedef Shape<128, 64, 4, 2, 3> DxFew;
+typedef Shape<128, 128, 4, 2, 2> DxSome;
+typedef Shape<256, 128, 8, 4, 3> DxMore;
+typedef Shape<256, 256, 8, 4, 2> DxMany;
+
+template <class S, int MODE>
+__global__ __launch_bounds__(S::threads) void head_logits_kernel(LogitArgs a)
 {
-	constexpr int WM = TT == 256 ? 2 : TT == 128 ? 4 : 8, WN = kHeadWaves / WM;
-	typedef Operand<true, true, kSide> W;
-	typedef Operand<false, false, TT> X;
-	constexpr int MB = kSide / WM / 32, NB = TT / WN / 32;
-	__shared__ __align__(16) char lds[2 * (W::kBytes + X::kBytes)];
+	constexpr int TT = S::tokens, TV = S::side;
+	constexpr int WM = S::waves_side, WN = S::waves_tokens;
+	typedef Operand<true, true, TV, S::threads> W;
+	typedef Operand<false, false, TT, S::threads> X;
+	constexpr int MB = TV / WM / 32, NB = TT / WN / 32;
+	__shared__ __align__(16) char lds[S::stages * (W::kBytes + X::kBytes)];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	int64_t tv, tt;
-	Product<W, X, MB, NB, false> prod;
+	Product<W, X, MB, NB, S::stages, false> prod;
 	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_t, &tv, &tt))
 		return;
-	const int64_t v_tile = a.v0 + tv * kSide;
+	const int64_t v_tile = a.v0 + tv * TV;
 	const int64_t t_tile = tt * TT;
 	const int64_t v_base = v_tile + wm * (MB * 32);
 
@@ -548,7 +608,7 @@ __global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
 				a.target_logit[t_tile + t] = hit;
 		}
 		__syncthreads();
-		for (int t = tid; t < TT; t += kHeadThreads) {
+		for (int t = tid; t < TT; t += S::threads) {
 			float top = -INFINITY, sum = 0.0f;
 
 #pragma unroll
@@ -601,7 +661,7 @@ __global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
 
 						w.x = bf16_rne2(acc[i][j][4 * q], acc[i][j][4 * q + 1]);
 						w.y = bf16_rne2(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
-						*(u32x2 *)(lds + t * (kSide * 2) + ((row >> 3) ^ (t & 31)) * 16 + (row & 4) * 2) = w;
+						*(u32x2 *)(lds + t * (TV * 2) + ((row >> 3) ^ (t & (TV / 8 - 1))) * 16 + (row & 4) * 2) = w;
 						if constexpr (MODE == kDeltaPair) {
 							/* what the rounding left over, for the second part */
 							acc[i][j][4 * q] -= __uint_as_float(w.x << 16);
@@ -612,12 +672,12 @@ __global__ __launch_bounds__(kHeadThreads) void head_logits_kernel(LogitArgs a)
 					}
 			__syncthreads();
 #pragma unroll
-			for (int c = tid; c < TT * (kSide / 8); c += kHeadThreads) {
-				const int t = c / (kSide / 8);
-				const int chunk = c % (kSide / 8);
+			for (int c = tid; c < TT * (TV / 8); c += S::threads) {
+				const int t = c / (TV / 8);
+				const int chunk = c % (TV / 8);
 
 				*(u32x4 *)(out + (t_tile + t) * a.ld_delta + (v_tile - a.v0) + chunk * 8) =
-				    *(const u32x4 *)(lds + t * (kSide * 2) + (chunk ^ (t & 31)) * 16);
+				    *(const u32x4 *)(lds + t * (TV * 2) + (chunk ^ (t & (TV / 8 - 1))) * 16);
 			}
 			if (part == 0 && MODE == kDeltaPair)
 				__syncthreads();
@@ -647,6 +707,7 @@ __global__ __launch_bounds__(kFinishWaves * 64) void head_finish_kernel(FinishAr
 	const int64_t t = (int64_t)blockIdx.x * 64 + lane;
 	float top = -INFINITY, sum = 0.0f;
 
+#pragma unroll 4
 	for (int64_t k = wave; k < a.tiles_v; k += kFinishWaves) {
 		const f32x2 p = a.part[k * a.rows_pad + t];
 		const float m = fmaxf(top, p.x);
@@ -690,14 +751,15 @@ struct DxArgs {
 };
 
 /* One slice of the contracted axis (the vocabulary) per blockIdx.y, each with a slot of its own. */
-template <int TT>
-__global__ __launch_bounds__(kHeadThreads) void head_dx_kernel(DxArgs a)
+template <class S>
+__global__ __launch_bounds__(S::threads) void head_dx_kernel(DxArgs a)
 {
-	constexpr int WM = 2, WN = kHeadWaves / WM;
-	typedef Operand<false, false, TT> D;
-	typedef Operand<false, true, kSide> W;
-	constexpr int MB = TT / WM / 32, NB = kSide / WN / 32;
-	__shared__ __align__(16) char lds[2 * (D::kBytes + W::kBytes)];
+	constexpr int TT = S::tokens, TD = S::side;
+	constexpr int WM = S::waves_tokens, WN = S::waves_side;
+	typedef Operand<false, false, TT, S::threads> D;
+	typedef Operand<false, true, TD, S::threads> W;
+	constexpr int MB = TT / WM / 32, NB = TD / WN / 32;
+	__shared__ __align__(16) char lds[S::stages * (D::kBytes + W::kBytes)];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -706,19 +768,19 @@ __global__ __launch_bounds__(kHeadThreads) void head_dx_kernel(DxArgs a)
 	const int from = (int)((int64_t)total * blockIdx.y / a.splits);
 	const int to = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
 	int64_t tt, td;
-	Product<D, W, MB, NB, false> prod;
+	Product<D, W, MB, NB, S::stages, false> prod;
 	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_t, a.tiles_d, &tt, &td))
 		return;
-	prod.run(a.delta, a.w, tt * TT, td * kSide, from, to, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, false);
+	prod.run(a.delta, a.w, tt * TT, td * TD, from, to, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, false);
 	/* a block at a time: its old values are all on their way before the first store */
 #pragma unroll
 	for (int i = 0; i < MB; i++)
 #pragma unroll
 		for (int j = 0; j < NB; j++) {
 			const int64_t t = tt * TT + wm * (MB * 32) + i * 32 + block_row(0, lane);
-			const int64_t c = td * kSide + wn * (NB * 32) + j * 32 + (lane & 31);
+			const int64_t c = td * TD + wn * (NB * 32) + j * 32 + (lane & 31);
 			float *p = a.slot + ((int64_t)blockIdx.y * a.rows_pad + t) * a.d_pad + c;
 			float old[16];
 
@@ -796,20 +858,25 @@ __device__ __forceinline__ void add_to(void *base, int64_t i, float x)
 		((uint16_t *)base)[i] = (uint16_t)bf16_rne(bf16_widen(((uint16_t *)base)[i]) + x);
 }
 
-template <int GT>
-__global__ __launch_bounds__(kHeadThreads) void head_dw_kernel(DwArgs a)
+/*
+** SIDE: of the tile both ways.  Few tokens leave little to contract and dw to read and write: smaller
+** tiles then, several workgroups to a compute unit, one at its products while others are at theirs.
+*/
+template <int SIDE, int GT>
+__global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwArgs a)
 {
-	constexpr int WM = 2, WN = kHeadWaves / WM;
-	typedef Operand<true, false, kSide> X;
-	typedef Operand<true, false, kSide> D;
-	constexpr int MB = kSide / WM / 32, NB = kSide / WN / 32;
+	constexpr int kThreadsHere = SIDE == 256 ? 512 : 256;
+	constexpr int WM = 2, WN = kThreadsHere / 64 / WM;
+	typedef Operand<true, false, SIDE, kThreadsHere> X;
+	typedef Operand<true, false, SIDE, kThreadsHere> D;
+	constexpr int MB = SIDE / WM / 32, NB = SIDE / WN / 32;
 	__shared__ __align__(16) char lds[2 * (X::kBytes + D::kBytes)];
 	const int tid = threadIdx.x;
 	const int lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	int64_t td, tv;
-	Product<X, D, MB, NB, true> prod;
+	Product<X, D, MB, NB, 2, true> prod;
 	auto &acc = prod.acc;
 
 	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_d, &tv, &td))
@@ -817,12 +884,12 @@ __global__ __launch_bounds__(kHeadThreads) void head_dw_kernel(DwArgs a)
 	/* the column sums: in the tiles of the first rows of x^T, by the wavefronts that hold the upper half */
 	const bool sums = a.db != nullptr && td == 0 && wm == 0;
 
-	prod.run(a.x, a.delta, td * kSide, tv * kSide, 0, a.steps * a.parts, a.steps, lds, wm * (MB * 32),
+	prod.run(a.x, a.delta, td * SIDE, tv * SIDE, 0, a.steps * a.parts, a.steps, lds, wm * (MB * 32),
 	    wn * (NB * 32), tid, sums);
 	if (sums && lane < 32) {
 #pragma unroll
 		for (int j = 0; j < NB; j++) {
-			const int64_t v = a.v0 + tv * kSide + wn * (NB * 32) + j * 32 + lane;
+			const int64_t v = a.v0 + tv * SIDE + wn * (NB * 32) + j * 32 + lane;
 
 			if (v < a.vocab)
 				add_to<GT>(a.db, v, prod.sum[j][0]);
@@ -836,9 +903,11 @@ __global__ __launch_bounds__(kHeadThreads) void head_dw_kernel(DwArgs a)
 	** where this is most of the work, took 620 us).
 	*/
 	constexpr int kWide = GT == kF32 ? 4 : 8;		/* elements in sixteen bytes */
-	constexpr int kHalf = kSide / 2;
-	constexpr int kAhead = 8;
-	float *const tile = (float *)lds;			/* [kHalf][kSide] */
+	constexpr int kHalf = SIDE / 2;
+	constexpr int kChunksOf = kHalf * SIDE / kWide / kThreadsHere;	/* of a lane, per half */
+	constexpr int kAhead = kChunksOf < 8 ? kChunksOf : 8;	/* of them on their way together */
+	static_assert(kHalf * SIDE / kWide % (kAhead * kThreadsHere) == 0, "whole rounds");
+	float *const tile = (float *)lds;			/* [kHalf][SIDE] */
 
 #pragma unroll
 	for (int h = 0; h < 2; h++) {
@@ -850,29 +919,29 @@ __global__ __launch_bounds__(kHeadThreads) void head_dw_kernel(DwArgs a)
 			for (int j = 0; j < NB; j++)
 #pragma unroll
 				for (int r = 0; r < 16; r++)
-					tile[(wm * (kHalf / 2) + i * 32 + block_row(r, lane)) * kSide + wn * (NB * 32) + j * 32
+					tile[(wm * (kHalf / 2) + i * 32 + block_row(r, lane)) * SIDE + wn * (NB * 32) + j * 32
 					    + (lane & 31)] = acc[h * (MB / 2) + i][j][r];
 		__syncthreads();
-		for (int c0 = tid; c0 < kHalf * kSide / kWide; c0 += kAhead * kHeadThreads) {
+		for (int c0 = tid; c0 < kHalf * SIDE / kWide; c0 += kAhead * kThreadsHere) {
 			u32x4 old[kAhead];
 
 #pragma unroll
 			for (int u = 0; u < kAhead; u++) {
-				const int c = c0 + u * kHeadThreads;
-				const int row = c / (kSide / kWide);
-				const int64_t k = td * kSide + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
-				const int64_t v = a.v0 + tv * kSide + c % (kSide / kWide) * kWide;
+				const int c = c0 + u * kThreadsHere;
+				const int row = c / (SIDE / kWide);
+				const int64_t k = td * SIDE + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
+				const int64_t v = a.v0 + tv * SIDE + c % (SIDE / kWide) * kWide;
 
 				if (k < a.d && v + kWide <= a.vocab)
 					old[u] = *(const u32x4_any *)((const char *)a.dw + (k * a.vocab + v) * (16 / kWide));
 			}
 #pragma unroll
 			for (int u = 0; u < kAhead; u++) {
-				const int c = c0 + u * kHeadThreads;
-				const int row = c / (kSide / kWide);
-				const int64_t k = td * kSide + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
-				const int64_t v = a.v0 + tv * kSide + c % (kSide / kWide) * kWide;
-				const float *x = tile + row * kSide + c % (kSide / kWide) * kWide;
+				const int c = c0 + u * kThreadsHere;
+				const int row = c / (SIDE / kWide);
+				const int64_t k = td * SIDE + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
+				const int64_t v = a.v0 + tv * SIDE + c % (SIDE / kWide) * kWide;
+				const float *x = tile + row * SIDE + c % (SIDE / kWide) * kWide;
 
 				if (k >= a.d)
 					continue;
@@ -909,11 +978,19 @@ __global__ __launch_bounds__(kHeadThreads) void head_dw_kernel(DwArgs a)
 constexpr int kOdd = 128;
 static_assert((kSide + kOdd) * 2 % 512 == 256, "lines of whole tiles, then 256 bytes");
 
+/*
+** What a tile of 128 tokens costs per token against one of 256, in hundredths (measured, see below).
+*/
+constexpr size_t kMoreCost = 115;
+
 struct HeadPlan {
-	int	tile_t;		/* tokens per tile */
+	int	tile_t;		/* tokens per tile: 64 few, 128 some or more, 256 many */
+	bool	small;		/* the shapes for few and some tokens */
+	int	tile_v, tile_d;	/* the other side of the tiles of the logits and of dx */
 	int64_t	rows_pad;
 	int	d_pad;
-	int64_t	tiles_v;	/* of the whole vocabulary */
+	int64_t	vocab_pad;
+	int64_t	tiles_v;	/* of the logits, over the whole vocabulary */
 	int64_t	piece;		/* vocabulary places per piece of delta, a multiple of kSide */
 	int64_t	ld_xs, ld_delta;
 	int	parts;		/* bf16 numbers per element of delta */
@@ -942,10 +1019,17 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	    || (grad_type != -1 && grad_type != ANNI_F32 && grad_type != ANNI_BF16))
 		return false;
 	memset(p, 0, sizeof(*p));
-	p->tile_t = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+	p->small = rows <= 128;
+	if (p->small)
+		p->tile_t = rows <= 64 ? 64 : 128;
+	else
+		p->tile_t = up((size_t)rows, 128) * kMoreCost < up((size_t)rows, 256) * 100 ? 128 : 256;
+	p->tile_v = p->small ? LogitsFew::side : kSide;
+	p->tile_d = p->small ? DxFew::side : kSide;
 	p->rows_pad = (int64_t)up((size_t)rows, (size_t)p->tile_t);
 	p->d_pad = (int)up((size_t)d, kSide);
-	p->tiles_v = (vocab + kSide - 1) / kSide;
+	p->vocab_pad = (int64_t)up((size_t)vocab, kSide);
+	p->tiles_v = (vocab + p->tile_v - 1) / p->tile_v;
 	p->parts = grad_type == ANNI_F32 ? 2 : 1;
 	p->ld_xs = p->d_pad + kOdd;
 	p->off_xs = at;
@@ -953,7 +1037,7 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	p->off_ts = at;
 	at = up(at + (size_t)p->rows_pad * 4, 256);
 	p->off_bs = at;
-	at = up(at + (size_t)p->tiles_v * kSide * 4, 256);
+	at = up(at + (size_t)p->vocab_pad * 4, 256);
 	p->off_part = at;
 	at = up(at + (size_t)p->tiles_v * p->rows_pad * 8, 256);
 	p->off_hit = at;
@@ -961,9 +1045,9 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	p->off_lse = at;
 	at = up(at + (size_t)p->rows_pad * 4, 256);
 	if (grad_type != -1) {
-		const int64_t whole = p->tiles_v * kSide;
+		const int64_t whole = p->vocab_pad;
 		const int64_t fit = (int64_t)(delta_most / ((size_t)p->rows_pad * 2 * p->parts)) / kSide * kSide;
-		const int64_t tiles = p->rows_pad / p->tile_t * (p->d_pad / kSide);
+		const int64_t tiles = p->rows_pad / p->tile_t * ((d + p->tile_d - 1) / p->tile_d);
 		int64_t steps;
 
 		const int64_t pieces = fit < kSide ? whole / kSide : (whole + fit - 1) / fit;
@@ -976,13 +1060,15 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		** Slices of the vocabulary in dx, each with a float slot for the whole of dx: the fewest that fill
 		** nine tenths of the compute units' turns, of at least sixteen steps each.
 		*/
+		const int64_t units = p->small ? 2 * kUnits : kUnits;	/* two small tiles to a compute unit */
+
 		p->splits = 1;
 		for (int k = 1; k <= 64 && k * 16 <= steps; k++) {
 			const int64_t groups = tiles * k;
-			const int64_t turns = (groups + kUnits - 1) / kUnits;
+			const int64_t turns = (groups + units - 1) / units;
 
 			p->splits = k;
-			if (groups * 10 >= turns * kUnits * 9)
+			if (groups * 10 >= turns * units * 9)
 				break;
 		}
 		p->off_delta = at;
@@ -1001,17 +1087,54 @@ static int rows_grid(int64_t items)
 	return (int)(g > 8192 ? 8192 : g < 1 ? 1 : g);
 }
 
-template <int MODE>
-static void logits_launch(hipStream_t st, int tile_t, const LogitArgs &a)
+template <class S, int MODE>
+static void logits_go(hipStream_t st, const LogitArgs &a)
 {
-	const dim3 grid((unsigned)up((size_t)(a.tiles_v * a.tiles_t), 8));
+	hipLaunchKernelGGL((head_logits_kernel<S, MODE>), dim3((unsigned)up((size_t)(a.tiles_v * a.tiles_t), 8)),
+	    dim3(S::threads), 0, st, a);
+}
 
-	if (tile_t == 64)
-		hipLaunchKernelGGL((head_logits_kernel<64, MODE>), grid, dim3(kHeadThreads), 0, st, a);
-	else if (tile_t == 128)
-		hipLaunchKernelGGL((head_logits_kernel<128, MODE>), grid, dim3(kHeadThreads), 0, st, a);
+template <int MODE>
+static void logits_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &a)
+{
+	if (p.small && p.tile_t == 64)
+		logits_go<LogitsFew, MODE>(st, a);
+	else if (p.small)
+		logits_go<LogitsSome, MODE>(st, a);
+	else if (p.tile_t == 128)
+		logits_go<LogitsMore, MODE>(st, a);
 	else
-		hipLaunchKernelGGL((head_logits_kernel<256, MODE>), grid, dim3(kHeadThreads), 0, st, a);
+		logits_go<LogitsMany, MODE>(st, a);
+}
+
+template <class S>
+static void dx_go(hipStream_t st, const DxArgs &a)
+{
+	hipLaunchKernelGGL(head_dx_kernel<S>, dim3((unsigned)up((size_t)(a.tiles_t * a.tiles_d), 8), (unsigned)a.splits),
+	    dim3(S::threads), 0, st, a);
+}
+
+static void dx_launch(hipStream_t st, const HeadPlan &p, const DxArgs &a)
+{
+	if (p.small && p.tile_t == 64)
+		dx_go<DxFew>(st, a);
+	else if (p.small)
+		dx_go<DxSome>(st, a);
+	else if (p.tile_t == 128)
+		dx_go<DxMore>(st, a);
+	else
+		dx_go<DxMany>(st, a);
+}
+
+template <int GT>
+static void dw_launch(hipStream_t st, const HeadPlan &p, const DwArgs &a)
+{
+	const dim3 grid((unsigned)up((size_t)(a.tiles_d * a.tiles_v), 8));
+
+	if (p.small)
+		hipLaunchKernelGGL((head_dw_kernel<128, GT>), grid, dim3(256), 0, st, a);
+	else
+		hipLaunchKernelGGL((head_dw_kernel<256, GT>), grid, dim3(512), 0, st, a);
 }
 
 static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
@@ -1035,7 +1158,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	ra.d = j.d;
 	ra.d_pad = p.d_pad;
 	ra.vocab = j.vocab;
-	ra.vocab_pad = p.tiles_v * kSide;
+	ra.vocab_pad = p.vocab_pad;
 	ra.bias = j.d_bias;
 	ra.xs = xs;
 	ra.ld_xs = p.ld_xs;
@@ -1061,7 +1184,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	la.rows_pad = p.rows_pad;
 	la.part = (f32x2 *)(work + p.off_part);
 	la.target_logit = (float *)(work + p.off_hit);
-	logits_launch<kStats>(st, p.tile_t, la);
+	logits_launch<kStats>(st, p, la);
 
 	memset(&fa, 0, sizeof(fa));
 	fa.part = la.part;
@@ -1083,16 +1206,16 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		DwArgs wa;
 
 		la.v0 = v0;
-		la.tiles_v = here / kSide;
+		la.tiles_v = here / p.tile_v;
 		la.lse = lse;
 		la.scale = (float)j.scale;
 		la.delta = delta;
 		la.delta_low = low;
 		la.ld_delta = p.ld_delta;
 		if (p.parts == 2)
-			logits_launch<kDeltaPair>(st, p.tile_t, la);
+			logits_launch<kDeltaPair>(st, p, la);
 		else
-			logits_launch<kDelta>(st, p.tile_t, la);
+			logits_launch<kDelta>(st, p, la);
 
 		memset(&wa, 0, sizeof(wa));
 		wa.x = la.x;
@@ -1105,8 +1228,8 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		wa.delta.depth = p.rows_pad;
 		wa.steps = (int)(p.rows_pad / kStep);
 		wa.parts = p.parts;
-		wa.tiles_d = p.d_pad / kSide;
-		wa.tiles_v = here / kSide;
+		wa.tiles_d = (j.d + (p.small ? 127 : 255)) / (p.small ? 128 : 256);
+		wa.tiles_v = here / (p.small ? 128 : 256);
 		wa.d = j.d;
 		wa.vocab = j.vocab;
 		wa.v0 = v0;
@@ -1114,13 +1237,11 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		wa.db = j.d_db;
 		if (!j.d_dw)
 			wa.tiles_d = 1;			/* only the tiles that sum */
-		const dim3 wgrid((unsigned)up((size_t)(wa.tiles_d * wa.tiles_v), 8));
-
 		if (j.d_dw || j.d_db) {
 			if (j.grad_type == ANNI_F32)
-				hipLaunchKernelGGL(head_dw_kernel<kF32>, wgrid, dim3(kHeadThreads), 0, st, wa);
+				dw_launch<kF32>(st, p, wa);
 			else
-				hipLaunchKernelGGL(head_dw_kernel<kBF16>, wgrid, dim3(kHeadThreads), 0, st, wa);
+				dw_launch<kBF16>(st, p, wa);
 		}
 		if (j.d_dx) {
 			memset(&xa, 0, sizeof(xa));
@@ -1136,19 +1257,12 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			xa.parts = p.parts;
 			xa.splits = p.splits;
 			xa.tiles_t = p.rows_pad / p.tile_t;
-			xa.tiles_d = p.d_pad / kSide;
+			xa.tiles_d = (j.d + p.tile_d - 1) / p.tile_d;	/* every tile has a valid row of w */
 			xa.slot = (float *)(work + p.off_slot);
 			xa.rows_pad = p.rows_pad;
 			xa.d_pad = p.d_pad;
 			xa.add = v0 > 0;
-			const dim3 grid((unsigned)up((size_t)(xa.tiles_t * xa.tiles_d), 8), (unsigned)p.splits);
-
-			if (p.tile_t == 64)
-				hipLaunchKernelGGL(head_dx_kernel<64>, grid, dim3(kHeadThreads), 0, st, xa);
-			else if (p.tile_t == 128)
-				hipLaunchKernelGGL(head_dx_kernel<128>, grid, dim3(kHeadThreads), 0, st, xa);
-			else
-				hipLaunchKernelGGL(head_dx_kernel<256>, grid, dim3(kHeadThreads), 0, st, xa);
+			dx_launch(st, p, xa);
 		}
 	}
 	if (grad && j.d_dx) {
