@@ -528,11 +528,11 @@ template <int SIDE_, int TOKENS_, int WAVES_, int WAVES_SIDE_, int STAGES_> stru
 ** of the largest tile that fits.  In between: half of it along the tokens.
 */
 typedef Shape<64, 64, 4, 2, 4> LogitsFew;
-typedef Shape<64, 128, 4, 2, 3> LogitsSome;
+typedef Shape<128, 128, 8, 4, 2> LogitsSome;
 typedef Shape<256, 128, 8, 4, 3> LogitsMore;
 typedef Shape<256, 256, 8, 2, 2> LogitsMany;
 typedef Shape<128, 64, 4, 2, 3> DxFew;
-typedef Shape<128, 128, 4, 2, 2> DxSome;
+typedef Shape<256, 128, 8, 4, 3> DxSome;
 typedef Shape<256, 128, 8, 4, 3> DxMore;
 typedef Shape<256, 256, 8, 4, 2> DxMany;
 
@@ -846,6 +846,9 @@ struct DwArgs {
 	int64_t		v0;
 	void		*dw;		/* [d][vocab] or NULL */
 	void		*db;		/* [vocab] or NULL */
+	int		splits;		/* slices of the tokens, blockIdx.y; more than one: into slots */
+	float		*slot;		/* [splits][slot_rows + 1][ld_slot], the last line for db */
+	int64_t		slot_rows, ld_slot;
 };
 
 /* base[i] += x */
@@ -884,8 +887,28 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 	/* the column sums: in the tiles of the first rows of x^T, by the wavefronts that hold the upper half */
 	const bool sums = a.db != nullptr && td == 0 && wm == 0;
 
-	prod.run(a.x, a.delta, td * SIDE, tv * SIDE, 0, a.steps * a.parts, a.steps, lds, wm * (MB * 32),
-	    wn * (NB * 32), tid, sums);
+	const int total = a.steps * a.parts;
+	const int from = (int)((int64_t)total * blockIdx.y / a.splits);
+	const int to = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
+
+	prod.run(a.x, a.delta, td * SIDE, tv * SIDE, from, to, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, sums);
+	if (a.splits > 1) {
+		float *slot = a.slot + (int64_t)blockIdx.y * (a.slot_rows + 1) * a.ld_slot;
+
+#pragma unroll
+		for (int j = 0; j < NB; j++) {
+			const int64_t c = tv * SIDE + wn * (NB * 32) + j * 32 + (lane & 31);
+
+			if (sums && lane < 32)
+				slot[a.slot_rows * a.ld_slot + c] = prod.sum[j][0];
+#pragma unroll
+			for (int i = 0; i < MB; i++)
+#pragma unroll
+				for (int r = 0; r < 16; r++)
+					slot[(td * SIDE + wm * (MB * 32) + i * 32 + block_row(r, lane)) * a.ld_slot + c] = acc[i][j][r];
+		}
+		return;
+	}
 	if (sums && lane < 32) {
 #pragma unroll
 		for (int j = 0; j < NB; j++) {
@@ -969,6 +992,38 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 	}
 }
 
+struct DwSumArgs {
+	const float	*slot;		/* [splits][slot_rows + 1][ld_slot] */
+	int		splits;
+	int64_t		slot_rows, ld_slot;
+	int		d, vocab;
+	int64_t		v0, count;	/* places of this piece */
+	void		*dw;
+	void		*db;
+};
+
+/* dw and db += the slots' sums in order: a line of dw (or db, the last) to a row of workgroups. */
+template <int GT>
+__global__ __launch_bounds__(kThreads) void head_dw_sum_kernel(DwSumArgs a)
+{
+	const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+
+	if (c >= a.count)
+		return;
+	for (int64_t r = blockIdx.y; r <= a.d; r += gridDim.y) {
+		const bool last = r == a.d;
+		const float *p = a.slot + (last ? a.slot_rows : r) * a.ld_slot + c;
+		float s = 0.0f;
+
+		if (last ? !a.db : !a.dw)
+			continue;
+#pragma unroll 8
+		for (int k = 0; k < a.splits; k++)
+			s += p[(int64_t)k * (a.slot_rows + 1) * a.ld_slot];
+		add_to<GT>(last ? a.db : a.dw, last ? a.v0 + c : r * a.vocab + a.v0 + c, s);
+	}
+}
+
 /* ---- plan -------------------------------------------------------------------------------------- */
 
 /*
@@ -995,13 +1050,21 @@ struct HeadPlan {
 	int64_t	ld_xs, ld_delta;
 	int	parts;		/* bf16 numbers per element of delta */
 	int	splits;		/* slices of the vocabulary in dx */
-	size_t	off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_slot;
+	int	side_w;		/* of dw's tiles */
+	int	splits_w;	/* slices of the tokens in dw */
+	int64_t	slot_rows_w;
+	size_t	off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_slot, off_slot_w;
 	size_t	bytes;
 };
 
 static size_t up(size_t x, size_t a)
 {
 	return (x + a - 1) / a * a;
+}
+
+static int64_t count(int64_t n, int64_t tile)
+{
+	return (n + tile - 1) / tile;
 }
 
 static const int kUnits = 256;		/* compute units of an MI355X, a workgroup of a large tile each */
@@ -1019,17 +1082,18 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	    || (grad_type != -1 && grad_type != ANNI_F32 && grad_type != ANNI_BF16))
 		return false;
 	memset(p, 0, sizeof(*p));
-	p->small = rows <= 128;
+	/* large tiles only where there are enough of them: half a turn of the compute units */
+	p->small = rows <= 128 || count(rows, 256) * count(vocab, kSide) * 2 < kUnits;
 	if (p->small)
-		p->tile_t = rows <= 64 ? 64 : 128;
+		p->tile_t = rows <= 64 || count(rows, 64) * count(vocab, LogitsFew::side) < 2 * kUnits ? 64 : 128;
 	else
 		p->tile_t = up((size_t)rows, 128) * kMoreCost < up((size_t)rows, 256) * 100 ? 128 : 256;
-	p->tile_v = p->small ? LogitsFew::side : kSide;
-	p->tile_d = p->small ? DxFew::side : kSide;
+	p->tile_v = !p->small ? kSide : p->tile_t == 64 ? LogitsFew::side : LogitsSome::side;
+	p->tile_d = !p->small ? kSide : p->tile_t == 64 ? DxFew::side : DxSome::side;
 	p->rows_pad = (int64_t)up((size_t)rows, (size_t)p->tile_t);
 	p->d_pad = (int)up((size_t)d, kSide);
 	p->vocab_pad = (int64_t)up((size_t)vocab, kSide);
-	p->tiles_v = (vocab + p->tile_v - 1) / p->tile_v;
+	p->tiles_v = count(vocab, p->tile_v);
 	p->parts = grad_type == ANNI_F32 ? 2 : 1;
 	p->ld_xs = p->d_pad + kOdd;
 	p->off_xs = at;
@@ -1047,7 +1111,7 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	if (grad_type != -1) {
 		const int64_t whole = p->vocab_pad;
 		const int64_t fit = (int64_t)(delta_most / ((size_t)p->rows_pad * 2 * p->parts)) / kSide * kSide;
-		const int64_t tiles = p->rows_pad / p->tile_t * ((d + p->tile_d - 1) / p->tile_d);
+		const int64_t tiles = p->rows_pad / p->tile_t * count(d, p->tile_d);
 		int64_t steps;
 
 		const int64_t pieces = fit < kSide ? whole / kSide : (whole + fit - 1) / fit;
@@ -1060,7 +1124,7 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		** Slices of the vocabulary in dx, each with a float slot for the whole of dx: the fewest that fill
 		** nine tenths of the compute units' turns, of at least sixteen steps each.
 		*/
-		const int64_t units = p->small ? 2 * kUnits : kUnits;	/* two small tiles to a compute unit */
+		const int64_t units = p->small ? 2 * kUnits : kUnits;	/* few tokens are bound by memory: more on its way */
 
 		p->splits = 1;
 		for (int k = 1; k <= 64 && k * 16 <= steps; k++) {
@@ -1071,10 +1135,31 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 			if (groups * 10 >= turns * units * 9)
 				break;
 		}
+		/*
+		** dw: tiles of 128 by two to a compute unit take about seven tenths of the time of a turn of the
+		** large ones (measured where either fills the chip), a quarter of the work each.
+		*/
+		{
+			const int64_t large = count(d, 256) * count(p->piece, 256);
+			const int64_t little = count(d, 128) * count(p->piece, 128);
+
+			p->side_w = count(little, 2 * kUnits) * 7 < count(large, kUnits) * 10 ? 128 : 256;
+			/* a small vocabulary and many tokens: slices of at least eight steps, while half the chip idles */
+			p->splits_w = 1;
+			while (little * p->splits_w * 2 <= kUnits && p->splits_w < 64
+			    && p->rows_pad / kStep * p->parts >= 16 * p->splits_w)
+				p->splits_w *= 2;
+			if (p->splits_w > 1)
+				p->side_w = 128;
+			p->slot_rows_w = count(d, 128) * 128;
+		}
 		p->off_delta = at;
 		at = up(at + (size_t)p->rows_pad * p->ld_delta * 2 * p->parts, 256);
 		p->off_slot = at;
 		at = up(at + (size_t)p->splits * p->rows_pad * p->d_pad * 4, 256);
+		p->off_slot_w = at;
+		if (p->splits_w > 1)
+			at = up(at + (size_t)p->splits_w * (p->slot_rows_w + 1) * p->piece * 4, 256);
 	}
 	p->bytes = at;
 	return true;
@@ -1129,12 +1214,29 @@ static void dx_launch(hipStream_t st, const HeadPlan &p, const DxArgs &a)
 template <int GT>
 static void dw_launch(hipStream_t st, const HeadPlan &p, const DwArgs &a)
 {
-	const dim3 grid((unsigned)up((size_t)(a.tiles_d * a.tiles_v), 8));
+	const dim3 grid((unsigned)up((size_t)(a.tiles_d * a.tiles_v), 8), (unsigned)a.splits);
 
-	if (p.small)
+	if (p.side_w == 128)
 		hipLaunchKernelGGL((head_dw_kernel<128, GT>), grid, dim3(256), 0, st, a);
 	else
 		hipLaunchKernelGGL((head_dw_kernel<256, GT>), grid, dim3(512), 0, st, a);
+	if (a.splits > 1) {
+		DwSumArgs s;
+
+		memset(&s, 0, sizeof(s));
+		s.slot = a.slot;
+		s.splits = a.splits;
+		s.slot_rows = a.slot_rows;
+		s.ld_slot = a.ld_slot;
+		s.d = a.d;
+		s.vocab = a.vocab;
+		s.v0 = a.v0;
+		s.count = a.vocab - a.v0 < p.piece ? a.vocab - a.v0 : p.piece;
+		s.dw = a.dw;
+		s.db = a.db;
+		hipLaunchKernelGGL(head_dw_sum_kernel<GT>, dim3((unsigned)count(s.count, kThreads),
+		    (unsigned)(a.d + 1 < 1024 ? a.d + 1 : 1024)), dim3(kThreads), 0, st, s);
+	}
 }
 
 static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
@@ -1228,13 +1330,17 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		wa.delta.depth = p.rows_pad;
 		wa.steps = (int)(p.rows_pad / kStep);
 		wa.parts = p.parts;
-		wa.tiles_d = (j.d + (p.small ? 127 : 255)) / (p.small ? 128 : 256);
-		wa.tiles_v = here / (p.small ? 128 : 256);
+		wa.tiles_d = count(j.d, p.side_w);
+		wa.tiles_v = here / p.side_w;
 		wa.d = j.d;
 		wa.vocab = j.vocab;
 		wa.v0 = v0;
 		wa.dw = j.d_dw;
 		wa.db = j.d_db;
+		wa.splits = p.splits_w;
+		wa.slot = (float *)(work + p.off_slot_w);
+		wa.slot_rows = p.slot_rows_w;
+		wa.ld_slot = p.piece;
 		if (!j.d_dw)
 			wa.tiles_d = 1;			/* only the tiles that sum */
 		if (j.d_dw || j.d_db) {
@@ -1257,7 +1363,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			xa.parts = p.parts;
 			xa.splits = p.splits;
 			xa.tiles_t = p.rows_pad / p.tile_t;
-			xa.tiles_d = (j.d + p.tile_d - 1) / p.tile_d;	/* every tile has a valid row of w */
+			xa.tiles_d = count(j.d, p.tile_d);	/* every tile has a valid row of w */
 			xa.slot = (float *)(work + p.off_slot);
 			xa.rows_pad = p.rows_pad;
 			xa.d_pad = p.d_pad;

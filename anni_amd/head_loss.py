@@ -16,13 +16,14 @@ class HeadLoss:
         if not need:
             raise ValueError("anni_head_loss refuses rows=%d d=%d vocab=%d grad_type=%d" % (rows, d, vocab, grad_type))
         self.work = DeviceBuffer(need)
+        self.job = _l.HeadJob()
+        self.job.rows, self.job.d, self.job.vocab, self.job.grad_type = rows, d, vocab, grad_type
+        self.job.d_work, self.job.work_bytes = self.work.ptr, self.work.nbytes
 
-    def _job(self, x, target, nll, scale, dx, ld_x, ld_dx):
-        j = _l.HeadJob()
-        j.rows, j.d, j.vocab = self.rows, self.d, self.vocab
-        j.d_x, j.ld_x, j.d_target, j.d_nll = x, ld_x or self.d, target, nll
-        j.scale, j.d_dx, j.ld_dx, j.grad_type = scale, dx, ld_dx or self.d, self.grad_type
-        j.d_work, j.work_bytes = self.work.ptr, self.work.nbytes
+    def _fill(self, x, target, nll, scale, dx, ld_x, ld_dx):
+        j = self.job
+        j.d_x, j.d_target, j.d_nll, j.scale, j.d_dx = x, target, nll, scale, dx
+        j.ld_x, j.ld_dx = ld_x or self.d, ld_dx or self.d
         return j
 
     def _done(self, rc):
@@ -34,13 +35,13 @@ class HeadLoss:
         """Device addresses: x, w bf16, bias float or None, target int32, nll float; dx is written, dw and db are added to."""
         if not self.grad and (dx or dw or db):
             raise ValueError("made for the loss alone")
-        j = self._job(x, target, nll, scale, dx, ld_x, ld_dx)
+        j = self._fill(x, target, nll, scale, dx, ld_x, ld_dx)
         j.d_w, j.d_bias, j.d_dw, j.d_db = w, bias, dw, db
         self._done(self.L.anni_head_loss(C.byref(j)))
 
     def run_on(self, opt, w_tensor, b_tensor, x, target, nll, scale=1.0, dx=None, ld_x=None, ld_dx=None):
         """The same on an LmAdam's head: weights from its twins, gradients into its gradient flat (grad=False: none)."""
-        j = self._job(x, target, nll, scale, dx, ld_x, ld_dx)
+        j = self._fill(x, target, nll, scale, dx, ld_x, ld_dx)
         self._done(self.L.anni_adam_head_loss(opt.h, w_tensor, -1 if b_tensor is None else b_tensor, C.byref(j),
                                               int(self.grad)))
 

@@ -134,6 +134,23 @@ def test_loss_and_gradients(gpu, rows, d, vocab, grad_type):
     assert same_bits(nll, c.dnll.get()) and same_bits(dx, c.ddx.get())
 
 
+@pytest.mark.parametrize("grad_type", [F32, BF16])
+@pytest.mark.parametrize("rows,d,vocab", [(2500, 64, 256), (1030, 130, 131), (3000, 300, 70)])
+def test_many_tokens_and_a_small_vocabulary(gpu, rows, d, vocab, grad_type):
+    """dw has too few tiles for the chip: the tokens are cut into slices whose sums are added in order."""
+    c = Case(rows, d, vocab, grad_type)
+    c.place()
+    plan = c.plan()
+    c.run(plan)
+    c.check()
+    full = c.outputs()
+    for parts in (("dw",), ("db",)):
+        c.place()
+        c.run(plan, parts=parts)
+        for name, got, a, b in zip(("dw", "db"), c.outputs()[2:], full[2:], (c.dw0, c.db0)):
+            assert same_bits(got, a if name in parts else b), name
+
+
 @pytest.mark.parametrize("rows,d,vocab", SIZES)
 def test_the_loss_alone_has_the_same_bits(gpu, rows, d, vocab):
     c = Case(rows, d, vocab, F32)
@@ -355,7 +372,7 @@ def test_refusals_on_an_arena(gpu):
     def tries(w, b, grad=True, width=d, **kw):
         opt = LmAdam([(d * vocab, 3), (vocab, 0), (77, 0)], **kw)
         plan.grad = grad
-        plan.d = width
+        plan.d = plan.job.d = width
         try:
             plan.run_on(opt, w, b, x.ptr, t.ptr, nll.ptr)
         finally:
