@@ -865,7 +865,7 @@ __device__ __forceinline__ void add_to(void *base, int64_t i, float x)
 ** SIDE: of the tile both ways.  Few tokens leave little to contract and dw to read and write: smaller
 ** tiles then, several workgroups to a compute unit, one at its products while others are at theirs.
 */
-template <int SIDE, int GT>
+template <int SIDE, int GT, bool SLICED>
 __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwArgs a)
 {
 	constexpr int kThreadsHere = SIDE == 256 ? 512 : 256;
@@ -888,11 +888,11 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 	const bool sums = a.db != nullptr && td == 0 && wm == 0;
 
 	const int total = a.steps * a.parts;
-	const int from = (int)((int64_t)total * blockIdx.y / a.splits);
-	const int to = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
+	const int from = SLICED ? (int)((int64_t)total * blockIdx.y / a.splits) : 0;
+	const int to = SLICED ? (int)((int64_t)total * (blockIdx.y + 1) / a.splits) : total;
 
 	prod.run(a.x, a.delta, td * SIDE, tv * SIDE, from, to, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, sums);
-	if (a.splits > 1) {
+	if constexpr (SLICED) {
 		float *slot = a.slot + (int64_t)blockIdx.y * (a.slot_rows + 1) * a.ld_slot;
 
 #pragma unroll
@@ -1216,10 +1216,12 @@ static void dw_launch(hipStream_t st, const HeadPlan &p, const DwArgs &a)
 {
 	const dim3 grid((unsigned)up((size_t)(a.tiles_d * a.tiles_v), 8), (unsigned)a.splits);
 
-	if (p.side_w == 128)
-		hipLaunchKernelGGL((head_dw_kernel<128, GT>), grid, dim3(256), 0, st, a);
+	if (a.splits > 1)
+		hipLaunchKernelGGL((head_dw_kernel<128, GT, true>), grid, dim3(256), 0, st, a);
+	else if (p.side_w == 128)
+		hipLaunchKernelGGL((head_dw_kernel<128, GT, false>), grid, dim3(256), 0, st, a);
 	else
-		hipLaunchKernelGGL((head_dw_kernel<256, GT>), grid, dim3(512), 0, st, a);
+		hipLaunchKernelGGL((head_dw_kernel<256, GT, false>), grid, dim3(512), 0, st, a);
 	if (a.splits > 1) {
 		DwSumArgs s;
 
