@@ -523,17 +523,16 @@ template <int SIDE_, int TOKENS_, int WAVES_, int WAVES_SIDE_, int STAGES_> stru
 };
 
 /*
-** Few tokens: the products are bound by reading w once.  Small tiles, so that there are workgroups for
-** all compute units and two or three to each, with three stages on their way.  Many tokens: two stages
-** of the largest tile that fits.  In between: half of it along the tokens.
+** Many: two stages of the largest tile that fits, one workgroup to a compute unit.  Some: a quarter of
+** it, two workgroups to a compute unit, where the large tiles would not fill the chip or w is read
+** more than it is computed with (few rows).  Few: a quarter again, where even those are too few.
+** head_plan() has the rule and what it goes by.
 */
 typedef Shape<64, 64, 4, 2, 4> LogitsFew;
 typedef Shape<128, 128, 8, 4, 2> LogitsSome;
-typedef Shape<256, 128, 8, 4, 3> LogitsMore;
 typedef Shape<256, 256, 8, 2, 2> LogitsMany;
 typedef Shape<128, 64, 4, 2, 3> DxFew;
 typedef Shape<256, 128, 8, 4, 3> DxSome;
-typedef Shape<256, 128, 8, 4, 3> DxMore;
 typedef Shape<256, 256, 8, 4, 2> DxMany;
 
 template <class S, int MODE>
@@ -1033,14 +1032,9 @@ __global__ __launch_bounds__(kThreads) void head_dw_sum_kernel(DwSumArgs a)
 constexpr int kOdd = 128;
 static_assert((kSide + kOdd) * 2 % 512 == 256, "lines of whole tiles, then 256 bytes");
 
-/*
-** What a tile of 128 tokens costs per token against one of 256, in hundredths (measured, see below).
-*/
-constexpr size_t kMoreCost = 115;
-
 struct HeadPlan {
-	int	tile_t;		/* tokens per tile: 64 few, 128 some or more, 256 many */
-	bool	small;		/* the shapes for few and some tokens */
+	int	tile_t;		/* tokens per tile: 64 few, 128 some, 256 many */
+	bool	small;		/* not many */
 	int	tile_v, tile_d;	/* the other side of the tiles of the logits and of dx */
 	int64_t	rows_pad;
 	int	d_pad;
@@ -1077,17 +1071,26 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 {
 	const size_t delta_most = (size_t)512 << 20;
 	size_t at = 0;
+	int64_t large, middle;
 
 	if (rows <= 0 || rows > kHeadMaxRows || d <= 0 || d > kHeadMaxD || vocab <= 0 || vocab > kHeadMaxVocab
 	    || (grad_type != -1 && grad_type != ANNI_F32 && grad_type != ANNI_BF16))
 		return false;
 	memset(p, 0, sizeof(*p));
-	/* large tiles only where there are enough of them: half a turn of the compute units */
-	p->small = rows <= 128 || count(rows, 256) * count(vocab, kSide) * 2 < kUnits;
-	if (p->small)
-		p->tile_t = rows <= 64 || count(rows, 64) * count(vocab, LogitsFew::side) < 2 * kUnits ? 64 : 128;
+	/*
+	** A turn of large tiles, one to each compute unit, takes ten; the middle ones six for the first two
+	** to each compute unit, and proportionally more beyond that.  Scoring, middle against large, in us:
+	** 777 x 331 x 10007 28.8 / 38.7, 512 x 1024 x 16384 30 / 38, 1024 x 1024 x 16384 50 / 43,
+	** 2048 x 1024 x 16384 86 / 76.  Small against middle: 512 x 512 x 4096 14.6 / 16.5,
+	** 64 x 1536 x 50000 69 / 63.
+	*/
+	large = count(rows, 256) * count(vocab, 256);
+	middle = count(rows, 128) * count(vocab, 128);
+	if (count(large, kUnits) * 10 * 2 * kUnits <= (middle > 2 * kUnits ? middle : 2 * kUnits) * 6)
+		p->tile_t = 256;
 	else
-		p->tile_t = up((size_t)rows, 128) * kMoreCost < up((size_t)rows, 256) * 100 ? 128 : 256;
+		p->tile_t = middle < kUnits ? 64 : 128;
+	p->small = p->tile_t != 256;
 	p->tile_v = !p->small ? kSide : p->tile_t == 64 ? LogitsFew::side : LogitsSome::side;
 	p->tile_d = !p->small ? kSide : p->tile_t == 64 ? DxFew::side : DxSome::side;
 	p->rows_pad = (int64_t)up((size_t)rows, (size_t)p->tile_t);
@@ -1182,12 +1185,10 @@ static void logits_go(hipStream_t st, const LogitArgs &a)
 template <int MODE>
 static void logits_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &a)
 {
-	if (p.small && p.tile_t == 64)
+	if (p.tile_t == 64)
 		logits_go<LogitsFew, MODE>(st, a);
-	else if (p.small)
-		logits_go<LogitsSome, MODE>(st, a);
 	else if (p.tile_t == 128)
-		logits_go<LogitsMore, MODE>(st, a);
+		logits_go<LogitsSome, MODE>(st, a);
 	else
 		logits_go<LogitsMany, MODE>(st, a);
 }
@@ -1201,12 +1202,10 @@ static void dx_go(hipStream_t st, const DxArgs &a)
 
 static void dx_launch(hipStream_t st, const HeadPlan &p, const DxArgs &a)
 {
-	if (p.small && p.tile_t == 64)
+	if (p.tile_t == 64)
 		dx_go<DxFew>(st, a);
-	else if (p.small)
-		dx_go<DxSome>(st, a);
 	else if (p.tile_t == 128)
-		dx_go<DxMore>(st, a);
+		dx_go<DxSome>(st, a);
 	else
 		dx_go<DxMany>(st, a);
 }
