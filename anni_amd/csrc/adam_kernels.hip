@@ -1085,19 +1085,24 @@ __device__ __forceinline__ Q8Block q8_narrow(f32x4 M, f32x4 V, uint32_t x0)
 
 /*
 ** A tile on the element-wise path with 8-bit moments: still a block per wavefront, four elements to
-** a lane, because the block's exponent needs all of them.  Elements behind the flat count as 0.  (With
+** a lane, because the block's exponent needs all of them.  Elements behind the flat count as 0.  A
+** tensor's attributes are looked up when an element crosses into it, not for each.  (With
 ** all four blocks' loads ahead of the first block's arithmetic the test model's step fell from 15.6 to
 ** 14.6 us, and the registers that took, 181 for 121, cost the 185M set 10 %: not done.)
 */
 template <int GT, bool DER>
 __device__ __forceinline__ void tile_slow_q8(const UpdateArgs &a, const TileInfo &t, double gs, int tid)
 {
+	int s = t.s;
+	int64_t s_end = a.segs ? a.segs[s].end : a.n;
+	uint32_t flags = t.flags;
+	float sc = t.sc;
+
 #pragma unroll 1
 	for (int u = 0; u < kQuadsPerTile; u++) {
 		const int64_t i0 = t.base + (int64_t)(u * kThreads + tid) * kQuad;
 		const int64_t blk = i0 / kQ8Block;
 		f32x4 M = {0.0f, 0.0f, 0.0f, 0.0f}, V = M;
-		int s = t.s;
 
 		if (t.base + (int64_t)(u * kThreads + (tid & ~63)) * kQuad >= t.end)
 			return;			/* the whole block lies behind the flat; the same in every lane */
@@ -1107,21 +1112,20 @@ __device__ __forceinline__ void tile_slow_q8(const UpdateArgs &a, const TileInfo
 #pragma unroll
 		for (int k = 0; k < kQuad; k++) {
 			const int64_t i = i0 + k;
-			uint32_t flags = a.uniform_flags;
-			float sc = 1.0f;
 
 			if (i >= t.end) {
 				M[k] = 0.0f;
 				V[k] = 0.0f;
 				continue;
 			}
-			if (a.segs) {
-				while (i >= a.segs[s].end)
-					s++;
+			if (i >= s_end) {
+				do
+					s_end = a.segs[++s].end;
+				while (i >= s_end);
 				flags = a.segs[s].flags;
+				if (GT == kFP8)
+					sc = a.gscale[s];
 			}
-			if (GT == kFP8)
-				sc = a.gscale[s];
 			const Elem e = adam_elem<true>(a.p[i], load_one<GT>(a.g, i, sc), M[k], V[k], gs, a.c,
 			    a.c.decay_on && (flags & kSegDecay) != 0);
 
