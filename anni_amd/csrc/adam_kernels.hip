@@ -1126,7 +1126,7 @@ __device__ __forceinline__ void tile_slow_q8(const UpdateArgs &a, const TileInfo
 				if (GT == kFP8)
 					sc = a.gscale[s];
 			}
-			const Elem e = adam_elem<true>(a.p[i], load_one<GT>(a.g, i, sc), M[k], V[k], gs, a.c,
+			const Elem e = adam_elem_near(a.p[i], load_one<GT>(a.g, i, sc), M[k], V[k], gs, a.c,
 			    a.c.decay_on && (flags & kSegDecay) != 0);
 
 			M[k] = e.m;
@@ -1274,8 +1274,8 @@ __device__ __forceinline__ void half_consume(const HalfStage<GT, MT> &st, const 
 
 #pragma unroll
 		for (int k = 0; k < kQuad; k++) {
-			const Elem e = adam_elem<(GT != kF32 || MT != kF32)>(P[k], G[k], M[k], V[k], gs, a.c,
-			    decay);
+			const Elem e = MT == kQ8 ? adam_elem_near(P[k], G[k], M[k], V[k], gs, a.c, decay)
+			    : adam_elem<(GT != kF32 || MT != kF32)>(P[k], G[k], M[k], V[k], gs, a.c, decay);
 
 			P[k] = e.p;
 			M[k] = e.m;

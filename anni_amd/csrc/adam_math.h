@@ -103,6 +103,55 @@ __device__ __forceinline__ Elem adam_elem(float p, float g, float m, float v, do
 	return r;
 }
 
+/*
+** The same for 8-bit moments.  m and v are the host loop's to the bit -- their codes hang on it --
+** but the step on p takes the products with 1/bc1 and 1/bc2 for the quotients and one Newton step
+** each behind the hardware's 23-bit reciprocal square root and reciprocal for the IEEE square root
+** and division: within 2^-43 of the host loop's step, which changes the float that p rounds to in about one
+** element of 10^8.  Those modes move 16 - 22 bytes per element and are bound by their vector
+** instructions (114 per element with the IEEE sequences, pipes busy all the time).
+*/
+__device__ __forceinline__ Elem adam_elem_near(float p, float g, float m, float v, double gs,
+	const StepConsts &c, bool decay)
+{
+	Elem r;
+	const double x = (double)g * gs;
+	double root, step;
+
+	r.m = (float)(c.beta1 * (double)m + c.omb1 * x);
+	r.v = (float)(c.beta2 * (double)v + (c.omb2 * x) * x);
+	{
+		/* 1e-300 is nothing to any float's quotient and keeps 0 from 0 * inf */
+		const double vhat = (double)r.v * c.rbc2 + 1e-300;
+		const double y = __builtin_amdgcn_rsq(vhat);
+		const double s = vhat * y;
+
+		root = __builtin_fma(__builtin_fma(-0.5 * y, s, 0.5), s, s);
+	}
+	{
+		const double d = root + c.eps;
+		const double y = __builtin_amdgcn_rcp(d);
+
+		step = (c.lr * ((double)r.m * c.rbc1)) * __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+	}
+	/* moments that are not finite: as the host loop divides them (see adam_elem) */
+	{
+		const bool odd = !__builtin_isfinite(__builtin_fabsf(r.m) + r.v);
+
+		if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
+			float fm = r.m, fv = r.v;
+
+			asm volatile("" : "+v"(fm), "+v"(fv));
+			if (odd)
+				step = (c.lr * ((double)fm / c.bc1)) / (sqrt((double)fv / c.bc2) + c.eps);
+		}
+	}
+	r.p = (float)((double)p - step);
+	if (decay)
+		r.p = (float)((double)r.p - c.lr_wd * (double)r.p);
+	return r;
+}
+
 /* float -> bfloat16 bits, round to nearest even; NaN stays NaN (quiet bit set). */
 __device__ __forceinline__ uint32_t bf16_rne(float x)
 {

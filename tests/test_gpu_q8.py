@@ -1,5 +1,6 @@
 """The arena with 8-bit moments (ANNI_Q8): every step against the C oracle on the decoded moments
-and the numpy model of the storage (q8_model.py), bit for bit."""
+and the numpy model of the storage (q8_model.py): codes and exponents bit for bit, p to a last place
+in at most a few elements (its step is within 2^-43, see near())."""
 import ctypes as C
 import tempfile
 
@@ -30,6 +31,17 @@ def new_arena(tensors, grad_type=F32, **kw):
     return LmAdam(tensors, grad_type=grad_type, moment_type=Q8, **kw), kw
 
 
+def near(got, want):
+    """The step on p is within 2^-43 of the host loop's, |step| <= lr (m and v of one history bound it by
+    a few lr) and p moves by less than 2^3 times itself here: the float it rounds to can be the
+    neighbour, when the exact value lies within 2^-43 |step| of the middle of two.  That is one
+    element in 2^43 ulp(p) / |step| > 2^17 for the smallest p of these tests and 10^8 for ordinary ones:
+    of the up to 70000 here at most three are let pass."""
+    same = got.view(np.uint32) == want.view(np.uint32)
+    return np.count_nonzero(~same) <= 3 and (np.abs(got.astype(np.float64) - want)
+                                             <= np.spacing(np.abs(want)))[~same].all()
+
+
 class Model:
     """Oracle + storage model of one arena."""
 
@@ -58,7 +70,9 @@ class Model:
 
     def check(self):
         o = self.opt
-        assert same_bits(o.download("param"), self.P)
+        got = o.download("param")
+        assert near(got, self.P)
+        self.P = got                        # the next step starts from the same p
         assert (o.download("m_exp") == self.bm).all() and (o.download("v_exp") == self.bv).all()
         assert (o.download("m") == self.cm).all() and (o.download("v") == self.cv).all()
         assert not o.download("grad").any()
