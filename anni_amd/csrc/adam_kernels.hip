@@ -1057,6 +1057,9 @@ __device__ __forceinline__ uint32_t amax4_bits(f32x4 x)
 struct Q8Block {
 	uint32_t	cm, cv;		/* four codes each */
 	uint32_t	b_m, b_v;
+
+	/* some moment is not finite (uniform) */
+	__device__ __forceinline__ bool odd(void) const { return b_m == 255u || b_v == 255u; }
 };
 
 __device__ __forceinline__ Q8Block q8_narrow(f32x4 M, f32x4 V, uint32_t x0)
@@ -1084,7 +1087,8 @@ __device__ __forceinline__ Q8Block q8_narrow(f32x4 M, f32x4 V, uint32_t x0)
 }
 
 /*
-** A tile on the element-wise path with 8-bit moments: still a block per wavefront, four elements to
+** A tile on the element-wise path with 8-bit moments (and the host loop's own step on p: this path
+** waits for memory, not for arithmetic): still a block per wavefront, four elements to
 ** a lane, because the block's exponent needs all of them.  Elements behind the flat count as 0.  A
 ** tensor's attributes are looked up when an element crosses into it, not for each.  (With
 ** all four blocks' loads ahead of the first block's arithmetic the test model's step fell from 15.6 to
@@ -1126,7 +1130,7 @@ __device__ __forceinline__ void tile_slow_q8(const UpdateArgs &a, const TileInfo
 				if (GT == kFP8)
 					sc = a.gscale[s];
 			}
-			const Elem e = adam_elem_near(a.p[i], load_one<GT>(a.g, i, sc), M[k], V[k], gs, a.c,
+			const Elem e = adam_elem<true>(a.p[i], load_one<GT>(a.g, i, sc), M[k], V[k], gs, a.c,
 			    a.c.decay_on && (flags & kSegDecay) != 0);
 
 			M[k] = e.m;
@@ -1272,17 +1276,15 @@ __device__ __forceinline__ void half_consume(const HalfStage<GT, MT> &st, const 
 			V = widen_raw<MT>(st.V[u], 1.0f);
 		}
 
-#pragma unroll
-		for (int k = 0; k < kQuad; k++) {
-			const Elem e = MT == kQ8 ? adam_elem_near(P[k], G[k], M[k], V[k], gs, a.c, decay)
-			    : adam_elem<(GT != kF32 || MT != kF32)>(P[k], G[k], M[k], V[k], gs, a.c, decay);
-
-			P[k] = e.p;
-			M[k] = e.m;
-			V[k] = e.v;
-		}
-		store_quad<kF32, NT>(a.p, idx, P);
 		if constexpr (MT == kQ8) {
+#pragma unroll
+			for (int k = 0; k < kQuad; k++) {
+				float m = M[k], v = V[k];
+
+				adam_moments(G[k], m, v, gs, a.c);
+				M[k] = m;
+				V[k] = v;
+			}
 			const Q8Block b = q8_narrow(M, V, (uint32_t)idx * kDitherGold + a.c.dither);
 
 			anni::st<NT>((uint32_t *)((uint8_t *)a.m + idx), b.cm);
@@ -1291,7 +1293,26 @@ __device__ __forceinline__ void half_consume(const HalfStage<GT, MT> &st, const 
 				a.m_exp[idx / kQ8Block] = (uint8_t)b.b_m;
 				a.v_exp[idx / kQ8Block] = (uint8_t)b.b_v;
 			}
+			if (__builtin_expect(b.odd(), 0)) {
+#pragma unroll
+				for (int k = 0; k < kQuad; k++)
+					P[k] = adam_step_near(P[k], M[k], V[k], a.c, decay, true);
+			} else {
+#pragma unroll
+				for (int k = 0; k < kQuad; k++)
+					P[k] = adam_step_near(P[k], M[k], V[k], a.c, decay, false);
+			}
+			store_quad<kF32, NT>(a.p, idx, P);
 		} else {
+#pragma unroll
+			for (int k = 0; k < kQuad; k++) {
+				const Elem e = adam_elem<(GT != kF32 || MT != kF32)>(P[k], G[k], M[k], V[k], gs, a.c, decay);
+
+				P[k] = e.p;
+				M[k] = e.m;
+				V[k] = e.v;
+			}
+			store_quad<kF32, NT>(a.p, idx, P);
 			store_quad<MT, NT>(a.m, idx, M);
 			store_quad<MT, NT>(a.v, idx, V);
 		}

@@ -104,52 +104,44 @@ __device__ __forceinline__ Elem adam_elem(float p, float g, float m, float v, do
 }
 
 /*
-** The same for 8-bit moments.  m and v are the host loop's to the bit -- their codes hang on it --
-** but the step on p takes the products with 1/bc1 and 1/bc2 for the quotients and one Newton step
-** each behind the hardware's 23-bit reciprocal square root and reciprocal for the IEEE square root
-** and division: within 2^-43 of the host loop's step, which changes the float that p rounds to in about one
-** element of 10^8.  Those modes move 16 - 22 bytes per element and are bound by their vector
-** instructions (114 per element with the IEEE sequences, pipes busy all the time).
+** The same for 8-bit moments, in two parts: the moments' codes are wanted between them.  m and v are
+** the host loop's to the bit -- the codes hang on it -- but the step on p takes the products with
+** 1/bc1 and 1/bc2 for the quotients and one Newton step each behind the hardware's 23-bit reciprocal
+** square root and reciprocal for the IEEE square root and division: within 2^-43 of the host loop's
+** step, which changes the float that p rounds to in about one element of 10^8.  Those modes move
+** 16 - 22 bytes per element and were bound by their vector instructions (114 per element with the
+** IEEE sequences, pipes busy all the time; 185M set 645 us with bf16 gradients).  `exact` (uniform):
+** some moment of the block is not finite, divide as the host loop does (see adam_elem).
 */
-__device__ __forceinline__ Elem adam_elem_near(float p, float g, float m, float v, double gs,
-	const StepConsts &c, bool decay)
+__device__ __forceinline__ void adam_moments(float g, float &m, float &v, double gs, const StepConsts &c)
 {
-	Elem r;
 	const double x = (double)g * gs;
-	double root, step;
 
-	r.m = (float)(c.beta1 * (double)m + c.omb1 * x);
-	r.v = (float)(c.beta2 * (double)v + (c.omb2 * x) * x);
-	{
+	m = (float)(c.beta1 * (double)m + c.omb1 * x);
+	v = (float)(c.beta2 * (double)v + (c.omb2 * x) * x);
+}
+
+__device__ __forceinline__ float adam_step_near(float p, float m, float v, const StepConsts &c, bool decay,
+	bool exact)
+{
+	double step;
+
+	if (exact) {
+		step = (c.lr * ((double)m / c.bc1)) / (sqrt((double)v / c.bc2) + c.eps);
+	} else {
 		/* 1e-300 is nothing to any float's quotient and keeps 0 from 0 * inf */
-		const double vhat = (double)r.v * c.rbc2 + 1e-300;
+		const double vhat = (double)v * c.rbc2 + 1e-300;
 		const double y = __builtin_amdgcn_rsq(vhat);
 		const double s = vhat * y;
+		const double d = __builtin_fma(__builtin_fma(-0.5 * y, s, 0.5), s, s) + c.eps;
+		const double z = __builtin_amdgcn_rcp(d);
 
-		root = __builtin_fma(__builtin_fma(-0.5 * y, s, 0.5), s, s);
+		step = (c.lr * ((double)m * c.rbc1)) * __builtin_fma(__builtin_fma(-d, z, 1.0), z, z);
 	}
-	{
-		const double d = root + c.eps;
-		const double y = __builtin_amdgcn_rcp(d);
-
-		step = (c.lr * ((double)r.m * c.rbc1)) * __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
-	}
-	/* moments that are not finite: as the host loop divides them (see adam_elem) */
-	{
-		const bool odd = !__builtin_isfinite(__builtin_fabsf(r.m) + r.v);
-
-		if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd) != 0, 0)) {
-			float fm = r.m, fv = r.v;
-
-			asm volatile("" : "+v"(fm), "+v"(fv));
-			if (odd)
-				step = (c.lr * ((double)fm / c.bc1)) / (sqrt((double)fv / c.bc2) + c.eps);
-		}
-	}
-	r.p = (float)((double)p - step);
+	p = (float)((double)p - step);
 	if (decay)
-		r.p = (float)((double)r.p - c.lr_wd * (double)r.p);
-	return r;
+		p = (float)((double)p - c.lr_wd * (double)p);
+	return p;
 }
 
 /* float -> bfloat16 bits, round to nearest even; NaN stays NaN (quiet bit set). */
