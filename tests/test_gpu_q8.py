@@ -197,6 +197,20 @@ def test_without_skip_a_gradient_that_is_not_finite_poisons_its_block(gpu, oracl
     opt.free()
 
 
+def test_without_eps_a_place_without_gradients_is_the_host_loops_nan(gpu, oracle):
+    tensors = [(4096 * 2 + 300, 3)]
+    opt, kw = new_arena(tensors, F32, eps=0.0, grad_clip=0.0)
+    rng = np.random.default_rng(16)
+    p = (rng.standard_normal(opt.n) * 0.02).astype(np.float32)
+    opt.upload("param", p)
+    g = (rng.standard_normal(opt.n) * 1e-3).astype(np.float32)
+    g[[5, 4100, 8400]] = 0.0
+    opt.upload("grad", g)
+    opt.step_scaled(1e-3)
+    assert np.flatnonzero(np.isnan(opt.download("param"))).tolist() == [5, 4100, 8400]
+    opt.free()
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_skipped_step_leaves_codes_and_exponents(gpu, oracle, bad):
     tensors = LISTS["ragged"]
