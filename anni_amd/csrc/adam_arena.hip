@@ -1476,6 +1476,38 @@ int anni_adam_read_state(anni_adam *opt, int fd, int *epoch, int *step)
 	return 0;
 }
 
+/* ---- the head's loss on the arena's own head ----------------------------------- */
+
+int anni_adam_head_loss(anni_adam *opt, int w_tensor, int b_tensor, const anni_head_job *job, int with_grad)
+{
+	anni_head_job j;
+	const Seg *w, *b = nullptr;
+	const size_t size = opt ? elem_bytes(opt->cfg.grad_type) : 0;
+
+	if (!opt || !opt->priv || !job || !opt->d_param_bf16 || job->d <= 0 || w_tensor < 0
+	    || w_tensor >= opt->n_tensors || b_tensor < -1 || b_tensor >= opt->n_tensors || b_tensor == w_tensor)
+		return -1;
+	w = &opt->priv->segs[(size_t)w_tensor];
+	if (b_tensor >= 0)
+		b = &opt->priv->segs[(size_t)b_tensor];
+	/* the step has to keep the twin, and the sizes have to fit */
+	if (!(w->flags & kSegTwin) || w->end == w->begin || (w->end - w->begin) % job->d != 0
+	    || (w->end - w->begin) / job->d > INT32_MAX || (b && (b->end - b->begin) * job->d != w->end - w->begin))
+		return -1;
+	if (with_grad && (opt->cfg.grad_type == ANNI_FP8_E4M3 || !opt->d_grad))
+		return -1;
+	j = *job;
+	j.vocab = (int)((w->end - w->begin) / job->d);
+	j.d_w = (const uint16_t *)opt->d_param_bf16 + w->begin;
+	j.d_bias = b ? opt->d_param + b->begin : nullptr;
+	j.grad_type = opt->cfg.grad_type;
+	j.d_dw = with_grad ? (char *)opt->d_grad + (size_t)w->begin * size : nullptr;
+	j.d_db = with_grad && b ? (char *)opt->d_grad + (size_t)b->begin * size : nullptr;
+	if (!with_grad)
+		j.d_dx = nullptr;
+	return anni_head_loss(&j);
+}
+
 /* ---- learning-rate schedule (lang/lm_train.c:98-124,398-411) ------------------ */
 
 static int g_warmup_steps;

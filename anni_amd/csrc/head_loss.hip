@@ -55,9 +55,8 @@ constexpr int kSide = 256;		/* of a result tile along the vocabulary or the mode
 ** read spread over all banks.
 **
 ** CHECK: the array ends inside tiles or its lines are not aligned to 16 bytes; such tiles go through
-** registers.  Loads never leave the array: what lies beyond along the contiguous axis reads as 0,
-** beyond along the other one the last valid line again (its product is with zeros, or not kept).
-** There has to be one: no tile or step is launched whose first line lies beyond the array.
+** registers.  Loads never leave the array, what lies beyond it reads as 0; no tile or step is
+** launched whose first line lies beyond.
 */
 struct Source {
 	const uint16_t	*part[2];	/* second: the low halves, same shape */
@@ -99,6 +98,7 @@ struct Operand {
 	uint32_t	offset;		/* elements from the tile's start to the lane's first chunk */
 	int		line, col;	/* its line, and its place in it */
 	u32x4		hold[CHECK ? kChunks : 1];
+	int		short_by;	/* lines from the lane's first to the end: what lies beyond is 0 */
 	bool		held;
 
 	static __device__ __forceinline__ int turn(int line)
@@ -180,6 +180,7 @@ struct Operand {
 					hold[i] = w;
 				}
 			}
+			short_by = lines - line;
 		}
 	}
 
@@ -190,7 +191,8 @@ struct Operand {
 			if (held)
 #pragma unroll
 				for (int i = 0; i < kChunks; i++)
-					*(u32x4 *)(lds + (tid + i * THREADS) * 16) = hold[i];
+					*(u32x4 *)(lds + (tid + i * THREADS) * 16) = i * kApart < short_by ? hold[i]
+					    : u32x4{0u, 0u, 0u, 0u};
 		}
 	}
 
@@ -1065,6 +1067,7 @@ static const int kUnits = 256;		/* compute units of an MI355X, a workgroup of a 
 static const int64_t kHeadMaxRows = (int64_t)1 << 22;
 static const int kHeadMaxD = 1 << 16;
 static const int kHeadMaxVocab = 1 << 22;
+static const int64_t kHeadMaxLogits = (int64_t)1 << 38;	/* 2^22 large tiles: what one launch may have */
 
 /* grad_type: -1 = the loss alone. */
 static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p)
@@ -1074,6 +1077,7 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	int64_t large, middle;
 
 	if (rows <= 0 || rows > kHeadMaxRows || d <= 0 || d > kHeadMaxD || vocab <= 0 || vocab > kHeadMaxVocab
+	    || rows * vocab > kHeadMaxLogits
 	    || (grad_type != -1 && grad_type != ANNI_F32 && grad_type != ANNI_BF16))
 		return false;
 	memset(p, 0, sizeof(*p));
@@ -1429,46 +1433,6 @@ int anni_head_loss(const anni_head_job *job)
 	if (!device_ready())
 		return -1;
 	return head_run(*job, p, grad);
-}
-
-int anni_adam_head_loss(anni_adam *opt, int w_tensor, int b_tensor, const anni_head_job *job, int with_grad)
-{
-	anni_head_job j;
-	int64_t w_at, w_n, b_at = 0, b_n;
-
-	if (!opt || !opt->priv || !job || !opt->d_param_bf16 || job->d <= 0 || w_tensor < 0
-	    || w_tensor >= opt->n_tensors || b_tensor < -1 || b_tensor >= opt->n_tensors)
-		return -1;
-	w_at = anni_adam_tensor_offset(opt, w_tensor);
-	w_n = (w_tensor + 1 < opt->n_tensors ? anni_adam_tensor_offset(opt, w_tensor + 1) : opt->n) - w_at;
-	if (w_n <= 0 || w_n % job->d != 0 || w_n / job->d > kHeadMaxVocab)
-		return -1;
-	j = *job;
-	j.vocab = (int)(w_n / job->d);
-	j.d_w = (const uint16_t *)opt->d_param_bf16 + w_at;
-	j.d_bias = nullptr;
-	if (b_tensor >= 0) {
-		b_at = anni_adam_tensor_offset(opt, b_tensor);
-		b_n = (b_tensor + 1 < opt->n_tensors ? anni_adam_tensor_offset(opt, b_tensor + 1) : opt->n) - b_at;
-		if (b_n != j.vocab)
-			return -1;
-		j.d_bias = opt->d_param + b_at;
-	}
-	j.grad_type = opt->cfg.grad_type;
-	j.d_dw = nullptr;
-	j.d_db = nullptr;
-	if (with_grad) {
-		const size_t size = opt->cfg.grad_type == ANNI_F32 ? 4 : 2;
-
-		if (opt->cfg.grad_type == ANNI_FP8_E4M3 || !opt->d_grad)
-			return -1;
-		j.d_dw = (char *)opt->d_grad + (size_t)w_at * size;
-		if (b_tensor >= 0)
-			j.d_db = (char *)opt->d_grad + (size_t)b_at * size;
-	} else {
-		j.d_dx = nullptr;
-	}
-	return anni_head_loss(&j);
 }
 
 } /* extern "C" */

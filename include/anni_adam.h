@@ -379,7 +379,7 @@ int	anni_colsum_add_batch(const anni_colsum *jobs, int n_jobs);
 ** the host.
 */
 typedef struct anni_head_job {
-	int64_t		rows;		/* up to 2^22 */
+	int64_t		rows;		/* up to 2^22, and rows * vocab up to 2^38 */
 	int		d;		/* up to 2^16 */
 	int		vocab;		/* up to 2^22 */
 	const void	*d_x;		/* bf16 */
@@ -401,11 +401,12 @@ typedef struct anni_head_job {
 size_t	anni_head_loss_work_bytes(int64_t rows, int d, int vocab, int grad_type);
 int	anni_head_loss(const anni_head_job *job);
 /*
-** The same on an arena: w is the twin of tensor w_tensor (d * vocab elements, vocab from
-** b_tensor's or w_tensor's size and d), b the float values of b_tensor (-1: none), and dw and db go
-** into the bound gradient flat.  x, targets, nll, scale, dx and the work area come from `job`, whose
-** vocab, d_w, d_bias, d_dw, d_db and grad_type are not read.  with_grad == 0: the loss alone.
-** -1 for gradients in an arena whose gradients are E4M3 codes (their scales are known only afterwards), or without twins.
+** The same on an arena: w is the twin of tensor w_tensor (flagged ANNI_T_TWIN; d * vocab elements,
+** which with job->d gives vocab), b the float values of b_tensor (vocab elements; -1: none), and dw
+** and db go into the bound gradient flat.  x, targets, nll, scale, dx and the work area come from
+** `job`, whose vocab, d_w, d_bias, d_dw, d_db and grad_type are not read.  with_grad == 0: the loss
+** alone.  -1 without twins, for tensors that do not fit, and for gradients in an arena whose
+** gradients are E4M3 codes (their scales are known only when the gradient is).
 */
 int	anni_adam_head_loss(anni_adam *opt, int w_tensor, int b_tensor, const anni_head_job *job, int with_grad);
 

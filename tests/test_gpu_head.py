@@ -229,6 +229,20 @@ def test_values_that_are_not_finite_reach_what_they_belong_to(gpu):
     assert np.isnan(dw).all() and np.isnan(db).all()
 
 
+def test_weights_that_are_not_finite(gpu):
+    """A column of -inf in the last lines of w (next to what pads the contracted axis): probability 0 or
+    1 by the sign of x, as the formula has it."""
+    c = Case(40, 70, 300, F32, pad=0.0, model=False)
+    c.x[:, 69] = np.where(np.arange(40) % 2, 0x3F80, 0x4000)        # 1 and 2
+    c.w[69, 17] = 0xFF80
+    c.target[c.target == 17] = 18
+    c.model()
+    c.place()
+    c.run(c.plan(False), grad=False)
+    c.check_nll()
+    assert np.isfinite(c.dnll.get()).all()
+
+
 def test_extreme_logits(gpu):
     """Logits of thousands: the maximum is subtracted before any exponential."""
     c = Case(33, 64, 600, F32, size=300.0)
@@ -383,7 +397,7 @@ def test_refusals_on_an_arena(gpu):
     tries(0, 1, grad=False, grad_type=FP8)
     for args, kw in (((0, 2), {}), ((0, 3), {}), ((-1, 1), {}), ((3, 1), {}), ((2, None), {}),
                      ((0, 1), dict(grad_type=FP8)), ((0, 1), dict(twins=False)), ((0, 1), dict(grad_slots=0)),
-                     ((0, 1), dict(width=15))):
+                     ((0, 1), dict(width=15)), ((0, 0), {}), ((1, None), dict(width=8)), ((1, None), dict(width=40))):
         with pytest.raises(RuntimeError):
             tries(*args, **kw)
     with pytest.raises(ValueError):

@@ -55,7 +55,8 @@ def test_work_area_sizes_and_refusals():
     assert f(1, 1, 1, -1) > 0 and f(1 << 22, 64, 256, lib.BF16) > 0
     for rows, d, vocab, ty in ((0, 8, 8, -1), (-1, 8, 8, -1), (8, 0, 8, -1), (8, 8, 0, -1), (8, 8, 8, -2),
                                (8, 8, 8, lib.FP8_E4M3), (8, 8, 8, lib.Q8), ((1 << 22) + 1, 8, 8, -1),
-                               (8, (1 << 16) + 1, 8, -1), (8, 8, (1 << 22) + 1, -1)):
+                               (8, (1 << 16) + 1, 8, -1), (8, 8, (1 << 22) + 1, -1),
+                               ((1 << 20) + 1, 8, 1 << 18, -1)):
         assert f(rows, d, vocab, ty) == 0
 
 
