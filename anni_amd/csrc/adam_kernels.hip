@@ -1293,8 +1293,8 @@ __device__ __forceinline__ void half_consume(const HalfStage<GT, MT> &st, const 
 				a.m_exp[idx / kQ8Block] = (uint8_t)b.b_m;
 				a.v_exp[idx / kQ8Block] = (uint8_t)b.b_v;
 			}
-			/* without an eps the host loop's 0 / 0 is a NaN: its own division then too */
-			if (__builtin_expect(b.odd() || !(a.c.eps > 0.0), 0)) {
+			/* 0 / 0 without an eps, x / inf with an endless one: the host loop's own division then too */
+			if (__builtin_expect(b.odd() || !(a.c.eps > 0.0 && a.c.eps < 1e100), 0)) {
 #pragma unroll
 				for (int k = 0; k < kQuad; k++)
 					P[k] = adam_step_near(P[k], M[k], V[k], a.c, decay, true);

@@ -211,6 +211,48 @@ def test_without_eps_a_place_without_gradients_is_the_host_loops_nan(gpu, oracle
     opt.free()
 
 
+def test_an_endless_eps_moves_nothing(gpu, oracle):
+    opt, kw = new_arena([(4096 * 2 + 300, 0)], F32, eps=np.inf, grad_clip=0.0)
+    rng = np.random.default_rng(17)
+    p = (rng.standard_normal(opt.n) * 0.02).astype(np.float32)
+    opt.upload("param", p)
+    opt.upload("grad", (rng.standard_normal(opt.n) * 1e-3).astype(np.float32))
+    opt.step_scaled(1e-3)
+    assert (opt.download("param") == p).all()
+    opt.free()
+
+
+@pytest.mark.parametrize("grad_type", [F32, BF16, FP8])
+def test_switches_change_no_bit(gpu, oracle, monkeypatch, grad_type):
+    """Tiles to a workgroup, the walk's direction, cache hints: 300 tiles, three steps each."""
+    tensors = [(4096 * 290, 3), (7, 0), (4096 * 10 + 77, 2)]
+    rng = np.random.default_rng(18)
+    n = sum(t[0] for t in tensors)
+    p = (rng.standard_normal(n) * 0.02).astype(np.float32)
+    data = [gradients(oracle, rng, tensors, grad_type, 1e-3) for _ in range(3)]
+    want = None
+    try:
+        for env in ({}, dict(ANNI_NT="0"), dict(ANNI_REVERSE="0", ANNI_KEEP_MB="0"), dict(ANNI_TILES_PER_WG="3"),
+                    dict(ANNI_TILES_PER_WG="0", ANNI_BLOCKS_PER_CU="1"), dict(ANNI_PIPE="0"), dict(ANNI_PIPE="2")):
+            with monkeypatch.context() as m:
+                for k, v in env.items():
+                    m.setenv(k, v)
+                gpu.anni_gpu_reload_switches()
+                opt, _kw = new_arena(tensors, grad_type, grad_clip=0.0)
+                opt.upload("param", p)
+                for g, scales in data:
+                    opt.upload("grad", g)
+                    if grad_type == FP8:
+                        opt.upload("gscale", scales)
+                    opt.step_scaled(1e-3)
+                got = [opt.download(k).tobytes() for k in ("param", "m", "v", "m_exp", "v_exp", "twin")]
+                opt.free()
+            want = want or got
+            assert got == want, env
+    finally:
+        gpu.anni_gpu_reload_switches()
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_skipped_step_leaves_codes_and_exponents(gpu, oracle, bad):
     tensors = LISTS["ragged"]
