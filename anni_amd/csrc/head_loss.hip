@@ -502,6 +502,8 @@ struct LogitArgs {
 	/* statistics */
 	f32x2		*part;		/* [tiles_v][rows_pad]: maximum, sum of exp(l - maximum) */
 	float		*target_logit;
+	f32x4		*kept;		/* the logits themselves, see kept_block(); NULL: nobody wants them */
+	int64_t		kept_v;		/* blocks along the vocabulary */
 	/* delta */
 	const float	*lse;
 	float		scale;
@@ -511,7 +513,16 @@ struct LogitArgs {
 	int64_t		ld_delta;
 };
 
-enum { kStats = 0, kDelta = 1, kDeltaPair = 2 };
+enum { kStats = 0, kDelta = 1, kDeltaPair = 2, kStatsKeep = 3 };
+
+/*
+** Logits that stay in memory lie as the accumulators do: blocks of 32 places by 32 tokens, four
+** sixteen-byte words per lane, so that they go out and come back in whole kilobytes.
+*/
+__device__ __forceinline__ f32x4 *kept_block(f32x4 *kept, int64_t kept_v, int64_t token, int64_t place)
+{
+	return kept + ((token / 32) * kept_v + place / 32) * 256;
+}
 
 /* A tile of VOCAB places and TOKENS tokens, or of the model's width and tokens, to a workgroup. */
 template <int SIDE_, int TOKENS_, int WAVES_, int WAVES_SIDE_, int STAGES_> struct Shape {
@@ -575,7 +586,20 @@ __global__ __launch_bounds__(S::threads) void head_logits_kernel(LogitArgs a)
 			if ((q & 1) == 1)
 				__builtin_amdgcn_sched_barrier(0);	/* all loads ahead of all sums take registers that there are not */
 		}
-	if constexpr (MODE == kStats) {
+	if constexpr (MODE == kStatsKeep) {
+#pragma unroll
+		for (int i = 0; i < MB; i++)
+#pragma unroll
+			for (int j = 0; j < NB; j++) {
+				f32x4 *block = kept_block(a.kept, a.kept_v, t_tile + wn * (NB * 32) + j * 32, v_base + i * 32);
+
+#pragma unroll
+				for (int q = 0; q < 4; q++)
+					__builtin_nontemporal_store(f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1],
+					    acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]}, block + q * 64 + lane);
+			}
+	}
+	if constexpr (MODE == kStats || MODE == kStatsKeep) {
 		f32x2 *red = (f32x2 *)lds;	/* [WM][TT] */
 
 #pragma unroll
@@ -736,6 +760,98 @@ __global__ __launch_bounds__(kFinishWaves * 64) void head_finish_kernel(FinishAr
 		a.lse[t] = top + log_sum;
 	if (t < a.rows)
 		a.nll[t] = live ? (top - a.target_logit[t]) + log_sum : 0.0f;
+}
+
+/* ---- delta from logits that were kept ------------------------------------------------------------ */
+
+struct DeltaArgs {
+	f32x4		*kept;
+	int64_t		kept_v;
+	const int32_t	*target;
+	const float	*lse;
+	float		scale;
+	int		vocab;
+	int64_t		v0;		/* of this piece */
+	int64_t		groups_v;	/* of 128 places, in this piece */
+	uint16_t	*delta;
+	uint16_t	*delta_low;
+	int64_t		ld_delta;
+};
+
+/*
+** 32 tokens by 128 places to a wavefront, four of them side by side: 16 KiB of logits on their way at
+** once, turned in LDS into lines of 256 bytes.
+*/
+template <bool PAIR>
+__global__ __launch_bounds__(kThreads) void head_delta_kernel(DeltaArgs a)
+{
+	__shared__ __align__(16) char lds[kThreads / 64][32 * 256];
+	const int lane = threadIdx.x & 63;
+	const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+	const int64_t unit = (int64_t)blockIdx.x * (kThreads / 64) + wave;	/* the grid divides them all */
+	const int64_t t0 = unit / a.groups_v * 32;
+	const int64_t c0 = unit % a.groups_v * 128;		/* from the piece's start */
+	const int64_t v_base = a.v0 + c0;
+	const int t = lane & 31;
+	const int target = a.target[t0 + t];
+	const float lse = a.lse[t0 + t];
+	const int want = target - (int)v_base - block_row(0, lane);
+	f32x4 x[4][4];
+
+#pragma unroll
+	for (int i = 0; i < 4; i++)
+#pragma unroll
+		for (int q = 0; q < 4; q++) {
+			/* blocks that lie beyond the vocabulary as a whole may not have been written */
+			x[i][q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+			if (v_base + i * 32 < a.vocab)
+				x[i][q] = __builtin_nontemporal_load(kept_block(a.kept, a.kept_v, t0, v_base + i * 32)
+				    + q * 64 + lane);
+		}
+#pragma unroll
+	for (int i = 0; i < 4; i++)
+#pragma unroll
+		for (int q = 0; q < 4; q++)
+#pragma unroll
+			for (int k = 0; k < 4; k++) {
+				float p = __expf(x[i][q][k] - lse);
+
+				if (want == i * 32 + 8 * q + k)
+					p -= 1.0f;
+				x[i][q][k] = target >= 0 && v_base + i * 32 < a.vocab ? p * a.scale : 0.0f;
+			}
+#pragma unroll
+	for (int part = 0; part < (PAIR ? 2 : 1); part++) {
+		uint16_t *out = (part ? a.delta_low : a.delta) + t0 * a.ld_delta + c0;
+
+#pragma unroll
+		for (int i = 0; i < 4; i++)
+#pragma unroll
+			for (int q = 0; q < 4; q++) {
+				u32x2 w;
+
+				w.x = bf16_rne2(x[i][q].x, x[i][q].y);
+				w.y = bf16_rne2(x[i][q].z, x[i][q].w);
+				*(u32x2 *)(lds[wave] + t * 256 + ((i * 4 + q) ^ (t & 15)) * 16 + (lane >> 5) * 8) = w;
+				if constexpr (PAIR) {
+					x[i][q].x -= __uint_as_float(w.x << 16);
+					x[i][q].y -= __uint_as_float(w.x & 0xffff0000u);
+					x[i][q].z -= __uint_as_float(w.y << 16);
+					x[i][q].w -= __uint_as_float(w.y & 0xffff0000u);
+				}
+			}
+		__syncthreads();
+#pragma unroll
+		for (int u = 0; u < 8; u++) {
+			const int line = u * 4 + (lane >> 4);
+			const int chunk = lane & 15;
+
+			*(u32x4 *)(out + line * a.ld_delta + chunk * 8) =
+			    *(const u32x4 *)(lds[wave] + line * 256 + (chunk ^ (line & 15)) * 16);
+		}
+		if (PAIR && part == 0)
+			__syncthreads();
+	}
 }
 
 /* ---- dx ---------------------------------------------------------------------------------------- */
@@ -1049,8 +1165,9 @@ struct HeadPlan {
 	int	side_w;		/* of dw's tiles */
 	int	splits_w;	/* slices of the tokens in dw */
 	int64_t	slot_rows_w;
-	size_t	off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_slot, off_slot_w;
-	size_t	bytes;
+	size_t	off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_kept, off_slot, off_slot_w;
+	size_t	bytes;		/* the least work area */
+	size_t	bytes_keep;	/* one that holds the logits between the passes */
 };
 
 static size_t up(size_t x, size_t a)
@@ -1073,6 +1190,7 @@ static const int64_t kHeadMaxLogits = (int64_t)1 << 38;	/* 2^22 large tiles: wha
 static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p)
 {
 	const size_t delta_most = (size_t)512 << 20;
+	const size_t kept_least = (size_t)512 << 20;	/* logits that are kept in any case: no more than a piece of delta */
 	size_t at = 0;
 	int64_t large, middle;
 
@@ -1168,7 +1286,15 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		if (p->splits_w > 1)
 			at = up(at + (size_t)p->splits_w * (p->slot_rows_w + 1) * p->piece * 4, 256);
 	}
-	p->bytes = at;
+	p->bytes = p->bytes_keep = at;
+	if (grad_type != -1) {
+		const size_t kept = (size_t)p->rows_pad * (size_t)p->vocab_pad * 4;
+
+		p->off_kept = at;
+		p->bytes_keep = at + kept;
+		if (kept <= kept_least)
+			p->bytes = p->bytes_keep;
+	}
 	return true;
 }
 
@@ -1189,12 +1315,42 @@ static void logits_go(hipStream_t st, const LogitArgs &a)
 template <int MODE>
 static void logits_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &a)
 {
-	if (p.tile_t == 64)
-		logits_go<LogitsFew, MODE>(st, a);
-	else if (p.tile_t == 128)
+	if constexpr (MODE == kStats || MODE == kStatsKeep)
+		if (p.tile_t == 64) {
+			logits_go<LogitsFew, MODE>(st, a);
+			return;
+		}
+	/* (the small tiles' logits are few enough to be kept: delta is never formed from them anew) */
+	if (p.tile_t == 128)
 		logits_go<LogitsSome, MODE>(st, a);
 	else
 		logits_go<LogitsMany, MODE>(st, a);
+}
+
+/* The same from the logits that were kept, for `here` places (a multiple of kSide) of the piece. */
+static void delta_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &l, int64_t here, int vocab)
+{
+	DeltaArgs a;
+
+	memset(&a, 0, sizeof(a));
+	a.kept = l.kept;
+	a.kept_v = l.kept_v;
+	a.target = l.target;
+	a.lse = l.lse;
+	a.scale = l.scale;
+	a.vocab = vocab;
+	a.v0 = l.v0;
+	a.groups_v = here / 128;
+	a.delta = l.delta;
+	a.delta_low = l.delta_low;
+	a.ld_delta = l.ld_delta;
+	/* at least two blocks of tokens and two groups: whole workgroups */
+	const dim3 grid((unsigned)(p.rows_pad / 32 * a.groups_v / (kThreads / 64)));
+
+	if (p.parts == 2)
+		hipLaunchKernelGGL(head_delta_kernel<true>, grid, dim3(kThreads), 0, st, a);
+	else
+		hipLaunchKernelGGL(head_delta_kernel<false>, grid, dim3(kThreads), 0, st, a);
 }
 
 template <class S>
@@ -1246,6 +1402,7 @@ static void dw_launch(hipStream_t st, const HeadPlan &p, const DwArgs &a)
 
 static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 {
+	const bool keep = grad && j.work_bytes >= p.bytes_keep;
 	hipStream_t st = compute_stream();
 	char *work = (char *)j.d_work;
 	uint16_t *xs = (uint16_t *)(work + p.off_xs);
@@ -1291,7 +1448,12 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	la.rows_pad = p.rows_pad;
 	la.part = (f32x2 *)(work + p.off_part);
 	la.target_logit = (float *)(work + p.off_hit);
-	logits_launch<kStats>(st, p, la);
+	la.kept = (f32x4 *)(work + p.off_kept);
+	la.kept_v = p.vocab_pad / 32;
+	if (keep)
+		logits_launch<kStatsKeep>(st, p, la);
+	else
+		logits_launch<kStats>(st, p, la);
 
 	memset(&fa, 0, sizeof(fa));
 	fa.part = la.part;
@@ -1319,7 +1481,9 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		la.delta = delta;
 		la.delta_low = low;
 		la.ld_delta = p.ld_delta;
-		if (p.parts == 2)
+		if (keep)
+			delta_launch(st, p, la, here, j.vocab);
+		else if (p.parts == 2)
 			logits_launch<kDeltaPair>(st, p, la);
 		else
 			logits_launch<kDelta>(st, p, la);
@@ -1409,6 +1573,13 @@ size_t anni_head_loss_work_bytes(int64_t rows, int d, int vocab, int grad_type)
 	HeadPlan p;
 
 	return head_plan(rows, d, vocab, grad_type, &p) ? p.bytes : 0;
+}
+
+size_t anni_head_loss_work_bytes_keep(int64_t rows, int d, int vocab, int grad_type)
+{
+	HeadPlan p;
+
+	return head_plan(rows, d, vocab, grad_type, &p) ? p.bytes_keep : 0;
 }
 
 int anni_head_loss(const anni_head_job *job)

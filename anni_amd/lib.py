@@ -141,6 +141,7 @@ _PROTOS = {
     "anni_fp8_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64]),
     "anni_colsum_add": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int]),
     "anni_head_loss_work_bytes": (C.c_size_t, [C.c_int64, C.c_int, C.c_int, C.c_int]),
+    "anni_head_loss_work_bytes_keep": (C.c_size_t, [C.c_int64, C.c_int, C.c_int, C.c_int]),
     "anni_head_loss": (C.c_int, [C.POINTER(HeadJob)]),
     "anni_adam_head_loss": (C.c_int, [C.POINTER(Adam), C.c_int, C.c_int, C.POINTER(HeadJob), C.c_int]),
     "anni_colsum_add_batch": (C.c_int, [C.POINTER(Colsum), C.c_int]),

@@ -356,7 +356,7 @@ int	anni_colsum_add_batch(const anni_colsum *jobs, int n_jobs);
 
 /*
 ** The head's loss: softmax cross entropy of logits = x w + b over the whole vocabulary, with its
-** gradients, without the logits in memory.  x is bf16 [rows][ld_x] (the last hidden states), w the
+** gradients; whole matrices of logits or probabilities need not fit into memory.  x is bf16 [rows][ld_x] (the last hidden states), w the
 ** bf16 [d][vocab] matrix the step keeps as the twin of w_head (lang/lm.c's logits = h w_head + b_head), b float [vocab]
 ** or NULL.
 **   nll[i] = log sum_v exp(l[i][v]) - l[i][target_i]
@@ -374,9 +374,10 @@ int	anni_colsum_add_batch(const anni_colsum *jobs, int n_jobs);
 **
 ** d_work: work_bytes of device memory, 256-byte aligned, at least anni_head_loss_work_bytes of the
 ** same sizes; nothing is kept in it between calls, and calls on different streams (or recorded
-** into graphs that may run at the same time) need one each.  It holds a copy of x, and for the gradients one
-** piece of delta of at most 512 MiB (more only if 256 places of the vocabulary need it).  Nothing else is allocated and nothing waits for
-** the host.
+** into graphs that may run at the same time) need one each.  It holds a copy of x, and for gradients
+** a piece of delta of at most 512 MiB (more only if 256 places of the vocabulary need it), what dx
+** is summed from (float, a copy for each slice of the vocabulary that works on it, up to 64 for small ones), the same for dw where the
+** vocabulary is small, and the logits if there is room.  Nothing else is allocated and nothing waits for the host.
 */
 typedef struct anni_head_job {
 	int64_t		rows;		/* up to 2^22, and rows * vocab up to 2^38 */
@@ -397,8 +398,14 @@ typedef struct anni_head_job {
 	void		*d_work;
 	size_t		work_bytes;
 } anni_head_job;
-/* grad_type -1: the loss alone.  0 for sizes or a type that are refused. */
+/*
+** grad_type -1: the loss alone.  0 for sizes or a type that are refused.  The first is the least; with
+** the second or more the logits of gradients stay in memory between the two passes (4 bytes for each of
+** rows * vocab, padded) instead of being computed again: the same bits sooner.  Up to 512 MiB of logits are part of the
+** first as well.
+*/
 size_t	anni_head_loss_work_bytes(int64_t rows, int d, int vocab, int grad_type);
+size_t	anni_head_loss_work_bytes_keep(int64_t rows, int d, int vocab, int grad_type);
 int	anni_head_loss(const anni_head_job *job);
 /*
 ** The same on an arena: w is the twin of tensor w_tensor (flagged ANNI_T_TWIN; d * vocab elements,

@@ -264,6 +264,37 @@ def test_several_pieces_of_the_vocabulary(gpu, rows, d, vocab, grad_type):
     c.check()
 
 
+@pytest.mark.parametrize("rows,d,vocab,grad_type", [(2100, 24, 60001, F32), (4097, 24, 65000, BF16),
+                                                    (300, 24, 350100, F32), (300, 24, 350100, BF16)])
+def test_logits_kept_or_computed_again_are_the_same_bits(gpu, rows, d, vocab, grad_type):
+    """More than 512 MiB of logits: the least work area has no room for them.  (300 tokens: middle tiles.)"""
+    from anni_amd.head_loss import HeadLoss
+    least = gpu.anni_head_loss_work_bytes(rows, d, vocab, grad_type)
+    most = gpu.anni_head_loss_work_bytes_keep(rows, d, vocab, grad_type)
+    assert most - least >= rows * vocab * 4
+    got = []
+    for keep, size in ((False, least), (True, most)):
+        c = Case(rows, d, vocab, grad_type, pad=0.3, model=False)
+        c.place()
+        plan = HeadLoss(rows, d, vocab, grad_type, keep=keep)
+        assert plan.work.nbytes == size
+        plan.work.upload(np.full(min(size, 1 << 30), 0xFF, np.uint8))
+        c.run(plan)
+        got.append([a.tobytes() for a in c.outputs()])
+        plan.free()
+    assert got[0] == got[1]
+
+
+def test_a_freed_plan_is_refused(gpu):
+    c = Case(8, 16, 40, F32, model=False)
+    c.place()
+    plan = c.plan()
+    c.run(plan)
+    plan.free()
+    with pytest.raises(RuntimeError):
+        c.run(plan)
+
+
 def test_work_area_contents_do_not_matter(gpu):
     c = Case(70, 72, 520, F32)
     c.place()

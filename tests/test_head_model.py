@@ -52,6 +52,9 @@ def test_work_area_sizes_and_refusals():
     loss, bf, f32 = (f(4096, 1536, 100000, t) for t in (-1, lib.BF16, lib.F32))
     assert 0 < loss < bf <= f32
     assert f32 < 4096 * 100000 * 4          # less than the logits it avoids
+    g = L.anni_head_loss_work_bytes_keep
+    assert g(4096, 1536, 100000, lib.BF16) >= bf + 4096 * 100000 * 4 and g(4096, 1536, 100000, -1) == loss
+    assert g(96, 1536, 100000, lib.BF16) == f(96, 1536, 100000, lib.BF16) and g(0, 8, 8, lib.F32) == 0
     assert f(1, 1, 1, -1) > 0 and f(1 << 22, 64, 256, lib.BF16) > 0
     for rows, d, vocab, ty in ((0, 8, 8, -1), (-1, 8, 8, -1), (8, 0, 8, -1), (8, 8, 0, -1), (8, 8, 8, -2),
                                (8, 8, 8, lib.FP8_E4M3), (8, 8, 8, lib.Q8), ((1 << 22) + 1, 8, 8, -1),
