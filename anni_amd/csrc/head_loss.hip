@@ -545,7 +545,8 @@ typedef Shape<64, 64, 4, 2, 4> LogitsFew;
 typedef Shape<128, 128, 8, 4, 2> LogitsSome;
 typedef Shape<256, 256, 8, 2, 2> LogitsMany;
 typedef Shape<128, 64, 4, 2, 3> DxFew;
-typedef Shape<256, 128, 8, 4, 3> DxSome;
+typedef Shape<128, 128, 8, 4, 2> DxSome;
+typedef Shape<256, 128, 8, 4, 3> DxOne;
 typedef Shape<256, 256, 8, 4, 2> DxMany;
 
 template <class S, int MODE>
@@ -779,79 +780,66 @@ struct DeltaArgs {
 };
 
 /*
-** 32 tokens by 128 places to a wavefront, four of them side by side: 16 KiB of logits on their way at
-** once, turned in LDS into lines of 256 bytes.
+** 32 tokens by 128 places to a workgroup, a block to a wavefront, turned in LDS into lines of 256
+** bytes.
 */
 template <bool PAIR>
 __global__ __launch_bounds__(kThreads) void head_delta_kernel(DeltaArgs a)
 {
-	__shared__ __align__(16) char lds[kThreads / 64][32 * 256];
-	const int lane = threadIdx.x & 63;
-	const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-	const int64_t unit = (int64_t)blockIdx.x * (kThreads / 64) + wave;	/* the grid divides them all */
-	const int64_t t0 = unit / a.groups_v * 32;
-	const int64_t c0 = unit % a.groups_v * 128;		/* from the piece's start */
-	const int64_t v_base = a.v0 + c0;
+	__shared__ __align__(16) char lds[PAIR ? 2 : 1][32 * 256];
+	const int tid = threadIdx.x;
+	const int lane = tid & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int64_t t0 = blockIdx.x / a.groups_v * 32;
+	const int64_t c0 = blockIdx.x % a.groups_v * 128;	/* from the piece's start */
+	const int64_t v_base = a.v0 + c0 + wave * 32;
 	const int t = lane & 31;
 	const int target = a.target[t0 + t];
 	const float lse = a.lse[t0 + t];
 	const int want = target - (int)v_base - block_row(0, lane);
-	f32x4 x[4][4];
+	/* blocks that lie beyond the vocabulary as a whole may not have been written */
+	const bool inside = v_base < a.vocab;
+	const f32x4 *block = kept_block(a.kept, a.kept_v, t0, inside ? v_base : 0) + lane;
+	f32x4 x[4];
+
+	static_assert(kThreads == 256, "four blocks of 32 places");
+#pragma unroll
+	for (int q = 0; q < 4; q++)
+		x[q] = __builtin_nontemporal_load(block + q * 64);
+#pragma unroll
+	for (int q = 0; q < 4; q++) {
+		const int chunk = (wave * 4 + q) ^ (t & 15);
+		u32x2 w;
 
 #pragma unroll
-	for (int i = 0; i < 4; i++)
-#pragma unroll
-		for (int q = 0; q < 4; q++) {
-			/* blocks that lie beyond the vocabulary as a whole may not have been written */
-			x[i][q] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-			if (v_base + i * 32 < a.vocab)
-				x[i][q] = __builtin_nontemporal_load(kept_block(a.kept, a.kept_v, t0, v_base + i * 32)
-				    + q * 64 + lane);
+		for (int k = 0; k < 4; k++) {
+			float p = __expf(x[q][k] - lse);
+
+			if (want == 8 * q + k)
+				p -= 1.0f;
+			x[q][k] = target >= 0 && inside ? p * a.scale : 0.0f;
 		}
-#pragma unroll
-	for (int i = 0; i < 4; i++)
-#pragma unroll
-		for (int q = 0; q < 4; q++)
-#pragma unroll
-			for (int k = 0; k < 4; k++) {
-				float p = __expf(x[i][q][k] - lse);
+		w.x = bf16_rne2(x[q].x, x[q].y);
+		w.y = bf16_rne2(x[q].z, x[q].w);
+		*(u32x2 *)(lds[0] + t * 256 + chunk * 16 + (lane >> 5) * 8) = w;
+		if constexpr (PAIR) {
+			const u32x2 low = {bf16_rne2(x[q].x - __uint_as_float(w.x << 16), x[q].y - __uint_as_float(w.x & 0xffff0000u)),
+			    bf16_rne2(x[q].z - __uint_as_float(w.y << 16), x[q].w - __uint_as_float(w.y & 0xffff0000u))};
 
-				if (want == i * 32 + 8 * q + k)
-					p -= 1.0f;
-				x[i][q][k] = target >= 0 && v_base + i * 32 < a.vocab ? p * a.scale : 0.0f;
-			}
-#pragma unroll
-	for (int part = 0; part < (PAIR ? 2 : 1); part++) {
-		uint16_t *out = (part ? a.delta_low : a.delta) + t0 * a.ld_delta + c0;
-
-#pragma unroll
-		for (int i = 0; i < 4; i++)
-#pragma unroll
-			for (int q = 0; q < 4; q++) {
-				u32x2 w;
-
-				w.x = bf16_rne2(x[i][q].x, x[i][q].y);
-				w.y = bf16_rne2(x[i][q].z, x[i][q].w);
-				*(u32x2 *)(lds[wave] + t * 256 + ((i * 4 + q) ^ (t & 15)) * 16 + (lane >> 5) * 8) = w;
-				if constexpr (PAIR) {
-					x[i][q].x -= __uint_as_float(w.x << 16);
-					x[i][q].y -= __uint_as_float(w.x & 0xffff0000u);
-					x[i][q].z -= __uint_as_float(w.y << 16);
-					x[i][q].w -= __uint_as_float(w.y & 0xffff0000u);
-				}
-			}
-		__syncthreads();
-#pragma unroll
-		for (int u = 0; u < 8; u++) {
-			const int line = u * 4 + (lane >> 4);
-			const int chunk = lane & 15;
-
-			*(u32x4 *)(out + line * a.ld_delta + chunk * 8) =
-			    *(const u32x4 *)(lds[wave] + line * 256 + (chunk ^ (line & 15)) * 16);
+			*(u32x2 *)(lds[1] + t * 256 + chunk * 16 + (lane >> 5) * 8) = low;
 		}
-		if (PAIR && part == 0)
-			__syncthreads();
 	}
+	__syncthreads();
+#pragma unroll
+	for (int part = 0; part < (PAIR ? 2 : 1); part++)
+#pragma unroll
+		for (int u = 0; u < 2; u++) {
+			const int line = u * 16 + (tid >> 4);
+			const int chunk = tid & 15;
+
+			*(u32x4 *)((part ? a.delta_low : a.delta) + (t0 + line) * a.ld_delta + c0 + chunk * 8) =
+			    *(const u32x4 *)(lds[part] + line * 256 + (chunk ^ (line & 15)) * 16);
+		}
 }
 
 /* ---- dx ---------------------------------------------------------------------------------------- */
@@ -1215,6 +1203,13 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	p->small = p->tile_t != 256;
 	p->tile_v = !p->small ? kSide : p->tile_t == 64 ? LogitsFew::side : LogitsSome::side;
 	p->tile_d = !p->small ? kSide : p->tile_t == 64 ? DxFew::side : DxSome::side;
+	/*
+	** dx of one tile of tokens is the reading of w: wider tiles then, which read delta half as often, with
+	** a step more on its way.  us, wide against narrow: 96 x 1536 x 100000 107 / 149, more tokens
+	** 256 x 1024 x 16384 23.6 / 21.5, 512 x 712 x 50257 116 / 75, 777 x 331 x 10007 55 / 31.
+	*/
+	if (p->tile_t == 128 && rows <= 128)
+		p->tile_d = DxOne::side;
 	p->rows_pad = (int64_t)up((size_t)rows, (size_t)p->tile_t);
 	p->d_pad = (int)up((size_t)d, kSide);
 	p->vocab_pad = (int64_t)up((size_t)vocab, kSide);
@@ -1344,8 +1339,7 @@ static void delta_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &l, 
 	a.delta = l.delta;
 	a.delta_low = l.delta_low;
 	a.ld_delta = l.ld_delta;
-	/* at least two blocks of tokens and two groups: whole workgroups */
-	const dim3 grid((unsigned)(p.rows_pad / 32 * a.groups_v / (kThreads / 64)));
+	const dim3 grid((unsigned)(p.rows_pad / 32 * a.groups_v));
 
 	if (p.parts == 2)
 		hipLaunchKernelGGL(head_delta_kernel<true>, grid, dim3(kThreads), 0, st, a);
@@ -1364,6 +1358,8 @@ static void dx_launch(hipStream_t st, const HeadPlan &p, const DxArgs &a)
 {
 	if (p.tile_t == 64)
 		dx_go<DxFew>(st, a);
+	else if (p.tile_t == 128 && p.tile_d == DxOne::side)
+		dx_go<DxOne>(st, a);
 	else if (p.tile_t == 128)
 		dx_go<DxSome>(st, a);
 	else
