@@ -1242,12 +1242,16 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		steps = p->piece / kStep * p->parts;
 		/*
 		** Slices of the vocabulary in dx, each with a float slot for the whole of dx: the fewest that fill
-		** nine tenths of the compute units' turns, of at least sixteen steps each.
+		** nine tenths of the compute units' turns, of at least sixteen steps each, or of two while the slots
+		** take no more than 8 MiB, which no one has to fetch from far (us, sixteen against two:
+		** 254 x 64 x 256 9.7 / 4.8, 100 x 256 x 2001 18 / 7, 700 x 300 x 2000 17.5 / 11.3).
 		*/
+		const size_t near_slots = (size_t)8 << 20;
+		const size_t slot = (size_t)p->rows_pad * (size_t)p->d_pad * 4;
 		const int64_t units = p->small ? 2 * kUnits : kUnits;	/* few tokens are bound by memory: more on its way */
 
 		p->splits = 1;
-		for (int k = 1; k <= 64 && k * 16 <= steps; k++) {
+		for (int k = 1; k <= 64 && (k * 16 <= steps || (k * 2 <= steps && (size_t)k * slot <= near_slots)); k++) {
 			const int64_t groups = tiles * k;
 			const int64_t turns = (groups + units - 1) / units;
 
