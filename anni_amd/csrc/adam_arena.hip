@@ -822,6 +822,7 @@ static void describe(const anni_adam *opt, Flat *f)
 		f->v_exp = (uint8_t *)f->v + moment_blocks(opt->n) * kQ8Block;
 	}
 	f->segs = pv->d_segs;
+	f->n_segs = opt->n_tensors;
 	f->tile_seg = pv->d_tile_seg;
 	f->gscale = opt->d_gscale;
 	if (pv->derived) {

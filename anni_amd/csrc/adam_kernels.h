@@ -84,6 +84,7 @@ struct Flat {
 	void		*g;
 	void		*m;
 	void		*v;
+	int		n_segs;		/* of segs; 0: unknown */
 	uint8_t		*m_exp;		/* 8-bit moments: the exponent byte of every block of kQ8Block elements */
 	uint8_t		*v_exp;
 	uint16_t	*twin;		/* may be NULL */

@@ -21,6 +21,7 @@ LISTS = {
     "block+1": [(257, 3)],
     "tile": [(4096, 3)],
     "ragged": [(5000, 3), (3, 0), (0, 3), (4096 * 3, 3), (1, 1), (8191, 2), (255, 3), (40001, 3), (1023, 0)],
+    "many": [(70, 3), (1, 0)] * 120 + [(4096 * 3, 3), (9, 2)],     # more tensors than helpers are started for
     "tails": [(70, 0)] * 40 + [(4096 * 2 + 5, 3)],
 }
 
