@@ -1301,10 +1301,17 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 			const int64_t little = count(d, 128) * count(p->piece, 128);
 
 			p->side_w = count(little, 2 * kUnits) * 7 < count(large, kUnits) * 10 ? 128 : 256;
-			/* a small vocabulary and many tokens: slices of at least eight steps, while half the chip idles */
+			/*
+			** Slices of the tokens while half the chip idles: of at least eight steps, or two while the slots
+			** are near as well (us, dw with its sum: 254 x 64 x 256 10.8 / 9.0, 500 x 128 x 1000 14.6 / 10.1,
+			** 900 x 100 x 1500 19.9 / 12).
+			*/
+			const size_t slot_w = (size_t)(count(d, 128) * 128 + 1) * (size_t)p->piece * 4;
+			const int64_t steps_w = p->rows_pad / kStep * p->parts;
+
 			p->splits_w = 1;
-			while (little * p->splits_w * 2 <= kUnits && p->splits_w < 64
-			    && p->rows_pad / kStep * p->parts >= 16 * p->splits_w)
+			while (little * p->splits_w * 2 <= kUnits && p->splits_w < 64 && (steps_w >= 16 * p->splits_w
+			    || (steps_w >= 4 * p->splits_w && 2 * (size_t)p->splits_w * slot_w <= near_slots)))
 				p->splits_w *= 2;
 			if (p->splits_w > 1)
 				p->side_w = 128;
