@@ -415,19 +415,24 @@ __device__ __forceinline__ int block_row(int r, int lane)
 }
 
 /*
-** Which tile a workgroup takes.  Consecutive workgroups go to the eight dies in turn, so die x gets
-** the x-th eighth of the list, and the list runs over bands of eight tiles of the short axis: what a
-** die works on at one time shares operands in its level-two cache.
+** Which tile a workgroup takes, and which of `slices` of its contracted axis.  Consecutive workgroups
+** go to the eight dies in turn, so die x gets the x-th eighth of the list, and the list runs, slice
+** by slice, over bands of eight tiles of the short axis: what a die works on at one time shares operands in its
+** level-two cache.
 */
-__device__ __forceinline__ bool tile_of(int64_t id, int64_t tiles_a, int64_t tiles_b, int64_t *ta, int64_t *tb)
+__device__ __forceinline__ bool tile_of(int64_t id, int64_t tiles_a, int64_t tiles_b, int slices, int64_t *ta,
+	int64_t *tb, int *slice)
 {
-	const int64_t n = tiles_a * tiles_b;
+	const int64_t tiles = tiles_a * tiles_b;
+	const int64_t n = tiles * slices;
 	const int64_t per = (n + 7) / 8;
-	const int64_t at = (id & 7) * per + (id >> 3);
+	int64_t at = (id & 7) * per + (id >> 3);
 	const int64_t band = 8 * tiles_a;
 
 	if ((id >> 3) >= per || at >= n)
 		return false;
+	*slice = (int)(at / tiles);
+	at -= *slice * tiles;
 	const int64_t g = at / band;
 	const int64_t in = at - g * band;
 	const int64_t wide = tiles_b - g * 8 < 8 ? tiles_b - g * 8 : 8;
@@ -546,7 +551,6 @@ typedef Shape<128, 128, 8, 4, 2> LogitsSome;
 typedef Shape<256, 256, 8, 2, 2> LogitsMany;
 typedef Shape<128, 64, 4, 2, 3> DxFew;
 typedef Shape<128, 128, 8, 4, 2> DxSome;
-typedef Shape<256, 128, 8, 4, 3> DxOne;
 typedef Shape<256, 256, 8, 4, 2> DxMany;
 
 template <class S, int MODE>
@@ -563,10 +567,11 @@ __global__ __launch_bounds__(S::threads) void head_logits_kernel(LogitArgs a)
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	int64_t tv, tt;
+	int whole;
 	Product<W, X, MB, NB, S::stages, false> prod;
 	auto &acc = prod.acc;
 
-	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_t, &tv, &tt))
+	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_t, 1, &tv, &tt, &whole))
 		return;
 	const int64_t v_tile = a.v0 + tv * TV;
 	const int64_t t_tile = tt * TT;
@@ -888,7 +893,7 @@ struct DxArgs {
 	int		add;		/* later pieces of the vocabulary add to the slots */
 };
 
-/* One slice of the contracted axis (the vocabulary) per blockIdx.y, each with a slot of its own. */
+/* Each slice of the contracted axis (the vocabulary) has a slot of its own. */
 template <class S>
 __global__ __launch_bounds__(S::threads) void head_dx_kernel(DxArgs a)
 {
@@ -903,14 +908,16 @@ __global__ __launch_bounds__(S::threads) void head_dx_kernel(DxArgs a)
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	const int total = a.steps * a.parts;
-	const int from = (int)((int64_t)total * blockIdx.y / a.splits);
-	const int to = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
 	int64_t tt, td;
+	int slice;
 	Product<D, W, MB, NB, S::stages, false> prod;
 	auto &acc = prod.acc;
 
-	if (!tile_of(blockIdx.x, a.tiles_t, a.tiles_d, &tt, &td))
+	if (!tile_of(blockIdx.x, a.tiles_t, a.tiles_d, a.splits, &tt, &td, &slice))
 		return;
+	const int from = (int)((int64_t)total * slice / a.splits);
+	const int to = (int)((int64_t)total * (slice + 1) / a.splits);
+
 	prod.run(a.delta, a.w, tt * TT, td * TD, from, to, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, false);
 	/* a block at a time: its old values are all on their way before the first store */
 #pragma unroll
@@ -919,7 +926,7 @@ __global__ __launch_bounds__(S::threads) void head_dx_kernel(DxArgs a)
 		for (int j = 0; j < NB; j++) {
 			const int64_t t = tt * TT + wm * (MB * 32) + i * 32 + block_row(0, lane);
 			const int64_t c = td * TD + wn * (NB * 32) + j * 32 + (lane & 31);
-			float *p = a.slot + ((int64_t)blockIdx.y * a.rows_pad + t) * a.d_pad + c;
+			float *p = a.slot + ((int64_t)slice * a.rows_pad + t) * a.d_pad + c;
 			float old[16];
 
 			if (a.add) {
@@ -984,7 +991,7 @@ struct DwArgs {
 	int64_t		v0;
 	void		*dw;		/* [d][vocab] or NULL */
 	void		*db;		/* [vocab] or NULL */
-	int		splits;		/* slices of the tokens, blockIdx.y; more than one: into slots */
+	int		splits;		/* slices of the tokens; more than one: into slots */
 	float		*slot;		/* [splits][slot_rows + 1][ld_slot], the last line for db */
 	int64_t		slot_rows, ld_slot;
 };
@@ -997,6 +1004,28 @@ __device__ __forceinline__ void add_to(void *base, int64_t i, float x)
 		((float *)base)[i] += x;
 	else
 		((uint16_t *)base)[i] = (uint16_t)bf16_rne(bf16_widen(((uint16_t *)base)[i]) + x);
+}
+
+/* The same for the first n of N neighbours: all loads ahead of the stores, which the compiler cannot tell apart. */
+template <int GT, int N>
+__device__ __forceinline__ void add_some(void *base, int64_t i, int64_t n, const float *x)
+{
+	float old[N];
+
+#pragma unroll
+	for (int e = 0; e < N; e++) {
+		old[e] = 0.0f;
+		if (e < n)
+			old[e] = GT == kF32 ? ((float *)base)[i + e] : bf16_widen(((uint16_t *)base)[i + e]);
+	}
+#pragma unroll
+	for (int e = 0; e < N; e++)
+		if (e < n) {
+			if constexpr (GT == kF32)
+				((float *)base)[i + e] = old[e] + x[e];
+			else
+				((uint16_t *)base)[i + e] = (uint16_t)bf16_rne(old[e] + x[e]);
+		}
 }
 
 /*
@@ -1017,21 +1046,22 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 	const int wm = wave / WN, wn = wave % WN;
 	int64_t td, tv;
+	int slice;
 	Product<X, D, MB, NB, 2, true> prod;
 	auto &acc = prod.acc;
 
-	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_d, &tv, &td))
+	if (!tile_of(blockIdx.x, a.tiles_v, a.tiles_d, SLICED ? a.splits : 1, &tv, &td, &slice))
 		return;
 	/* the column sums: in the tiles of the first rows of x^T, by the wavefronts that hold the upper half */
 	const bool sums = a.db != nullptr && td == 0 && wm == 0;
 
 	const int total = a.steps * a.parts;
-	const int from = SLICED ? (int)((int64_t)total * blockIdx.y / a.splits) : 0;
-	const int to = SLICED ? (int)((int64_t)total * (blockIdx.y + 1) / a.splits) : total;
+	const int from = SLICED ? (int)((int64_t)total * slice / a.splits) : 0;
+	const int to = SLICED ? (int)((int64_t)total * (slice + 1) / a.splits) : total;
 
 	prod.run(a.x, a.delta, td * SIDE, tv * SIDE, from, to, a.steps, lds, wm * (MB * 32), wn * (NB * 32), tid, sums);
 	if constexpr (SLICED) {
-		float *slot = a.slot + (int64_t)blockIdx.y * (a.slot_rows + 1) * a.ld_slot;
+		float *slot = a.slot + (int64_t)slice * (a.slot_rows + 1) * a.ld_slot;
 
 #pragma unroll
 		for (int j = 0; j < NB; j++) {
@@ -1121,9 +1151,7 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 					}
 					*(u32x4_any *)((char *)a.dw + (k * a.vocab + v) * (16 / kWide)) = w;
 				} else {
-					for (int e = 0; e < kWide; e++)
-						if (v + e < a.vocab)
-							add_to<GT>(a.dw, k * a.vocab + v + e, x[e]);
+					add_some<GT, kWide>(a.dw, k * a.vocab + v, a.vocab - v, x);
 				}
 			}
 		}
@@ -1171,10 +1199,14 @@ __global__ __launch_bounds__(kThreads) void head_dw_sum_kernel(DwSumArgs a)
 constexpr int kOdd = 128;
 static_assert((kSide + kOdd) * 2 % 512 == 256, "lines of whole tiles, then 256 bytes");
 
+enum { kDxFew, kDxSome, kDxMany };
+
 struct HeadPlan {
 	int	tile_t;		/* tokens per tile: 64 few, 128 some, 256 many */
 	bool	small;		/* not many */
-	int	tile_v, tile_d;	/* the other side of the tiles of the logits and of dx */
+	int	tile_v;		/* the other side of the logits' tiles */
+	int	dx;		/* kDxFew .. kDxMany */
+	int	dx_t, tile_d;	/* its tiles */
 	int64_t	rows_pad;
 	int	d_pad;
 	int64_t	vocab_pad;
@@ -1187,6 +1219,7 @@ struct HeadPlan {
 	int	splits_w;	/* slices of the tokens in dw */
 	int64_t	slot_rows_w;
 	size_t	off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_kept, off_slot, off_slot_w;
+	bool	keeps;		/* the logits, if there is room */
 	size_t	bytes;		/* the least work area */
 	size_t	bytes_keep;	/* one that holds the logits between the passes */
 };
@@ -1235,14 +1268,15 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		p->tile_t = middle < kUnits ? 64 : 128;
 	p->small = p->tile_t != 256;
 	p->tile_v = !p->small ? kSide : p->tile_t == 64 ? LogitsFew::side : LogitsSome::side;
-	p->tile_d = !p->small ? kSide : p->tile_t == 64 ? DxFew::side : DxSome::side;
 	/*
-	** dx of one tile of tokens is the reading of w: wider tiles then, which read delta half as often, with
-	** a step more on its way.  us, wide against narrow: 96 x 1536 x 100000 107 / 149, more tokens
-	** 256 x 1024 x 16384 23.6 / 21.5, 512 x 712 x 50257 116 / 75, 777 x 331 x 10007 55 / 31.
+	** dx: small tiles with the small ones of the logits, middle ones with the middle ones, and also where
+	** the large ones would mostly cover what is not there: the middle ones take a third longer for the
+	** same area (us, large against middle: 4096 x 331 x 16384 f32 167 / 174, 2314 x 64 x 69760 bf16 140 / 90).
 	*/
-	if (p->tile_t == 128 && rows <= 128)
-		p->tile_d = DxOne::side;
+	p->dx = p->tile_t == 64 ? kDxFew : p->small
+	    || count(rows, 128) * count(d, 128) * 10 < count(rows, 256) * count(d, 256) * 28 ? kDxSome : kDxMany;
+	p->dx_t = p->dx == kDxFew ? DxFew::tokens : p->dx == kDxMany ? DxMany::tokens : DxSome::tokens;
+	p->tile_d = p->dx == kDxFew ? DxFew::side : p->dx == kDxMany ? DxMany::side : DxSome::side;
 	p->rows_pad = (int64_t)up((size_t)rows, (size_t)p->tile_t);
 	p->d_pad = (int)up((size_t)d, kSide);
 	p->vocab_pad = (int64_t)up((size_t)vocab, kSide);
@@ -1264,7 +1298,7 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	if (grad_type != -1) {
 		const int64_t whole = p->vocab_pad;
 		const int64_t fit = (int64_t)(delta_most / ((size_t)p->rows_pad * 2 * p->parts)) / kSide * kSide;
-		const int64_t tiles = p->rows_pad / p->tile_t * count(d, p->tile_d);
+		const int64_t tiles = p->rows_pad / p->dx_t * count(d, p->tile_d);
 		int64_t steps;
 
 		const int64_t pieces = fit < kSide ? whole / kSide : (whole + fit - 1) / fit;
@@ -1281,10 +1315,10 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		*/
 		const size_t near_slots = (size_t)8 << 20;
 		const size_t slot = (size_t)p->rows_pad * (size_t)p->d_pad * 4;
-		const int64_t units = p->small ? 2 * kUnits : kUnits;	/* few tokens are bound by memory: more on its way */
+		const int64_t units = p->dx == kDxMany ? kUnits : 2 * kUnits;	/* few tokens are bound by memory: more on its way */
 
 		p->splits = 1;
-		for (int k = 1; k <= 64 && (k * 16 <= steps || (k * 2 <= steps && (size_t)k * slot <= near_slots)); k++) {
+		for (int k = 1; k <= 256 && (k * 16 <= steps || (k * 2 <= steps && (size_t)k * slot <= near_slots)); k++) {
 			const int64_t groups = tiles * k;
 			const int64_t turns = (groups + units - 1) / units;
 
@@ -1329,10 +1363,18 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	if (grad_type != -1) {
 		const size_t kept = (size_t)p->rows_pad * (size_t)p->vocab_pad * 4;
 
-		p->off_kept = at;
-		p->bytes_keep = at + kept;
-		if (kept <= kept_least)
-			p->bytes = p->bytes_keep;
+		/*
+		** Keeping them writes and reads 8 bytes for each, computing them again takes 2 d operations.  us of
+		** the two passes, kept / again: 2048 x 128 x 32768 155 / 132, 2048 x 256 x 32768 175 / 188,
+		** 161 x 64 x 50304 34 / 28, 200 x 256 x 50304 33 / 38.  (The small tiles' are always kept: few.)
+		*/
+		if (d >= 192 || p->tile_t == 64) {
+			p->off_kept = at;
+			p->bytes_keep = at + kept;
+			p->keeps = true;
+			if (kept <= kept_least)
+				p->bytes = p->bytes_keep;
+		}
 	}
 	return true;
 }
@@ -1394,17 +1436,15 @@ static void delta_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &l, 
 template <class S>
 static void dx_go(hipStream_t st, const DxArgs &a)
 {
-	hipLaunchKernelGGL(head_dx_kernel<S>, dim3((unsigned)up((size_t)(a.tiles_t * a.tiles_d), 8), (unsigned)a.splits),
+	hipLaunchKernelGGL(head_dx_kernel<S>, dim3((unsigned)up((size_t)(a.tiles_t * a.tiles_d * a.splits), 8)),
 	    dim3(S::threads), 0, st, a);
 }
 
 static void dx_launch(hipStream_t st, const HeadPlan &p, const DxArgs &a)
 {
-	if (p.tile_t == 64)
+	if (p.dx == kDxFew)
 		dx_go<DxFew>(st, a);
-	else if (p.tile_t == 128 && p.tile_d == DxOne::side)
-		dx_go<DxOne>(st, a);
-	else if (p.tile_t == 128)
+	else if (p.dx == kDxSome)
 		dx_go<DxSome>(st, a);
 	else
 		dx_go<DxMany>(st, a);
@@ -1413,7 +1453,7 @@ static void dx_launch(hipStream_t st, const HeadPlan &p, const DxArgs &a)
 template <int GT>
 static void dw_launch(hipStream_t st, const HeadPlan &p, const DwArgs &a)
 {
-	const dim3 grid((unsigned)up((size_t)(a.tiles_d * a.tiles_v), 8), (unsigned)a.splits);
+	const dim3 grid((unsigned)up((size_t)(a.tiles_d * a.tiles_v * a.splits), 8));
 
 	if (a.splits > 1)
 		hipLaunchKernelGGL((head_dw_kernel<128, GT, true>), grid, dim3(256), 0, st, a);
@@ -1442,7 +1482,7 @@ static void dw_launch(hipStream_t st, const HeadPlan &p, const DwArgs &a)
 
 static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 {
-	const bool keep = grad && j.work_bytes >= p.bytes_keep;
+	const bool keep = grad && p.keeps && j.work_bytes >= p.bytes_keep;
 	hipStream_t st = compute_stream();
 	char *work = (char *)j.d_work;
 	uint16_t *xs = (uint16_t *)(work + p.off_xs);
@@ -1572,7 +1612,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			xa.steps = (int)((left < here ? left : here) + kStep - 1) / kStep;
 			xa.parts = p.parts;
 			xa.splits = p.splits;
-			xa.tiles_t = p.rows_pad / p.tile_t;
+			xa.tiles_t = p.rows_pad / p.dx_t;
 			xa.tiles_d = count(j.d, p.tile_d);	/* every tile has a valid row of w */
 			xa.slot = (float *)(work + p.off_slot);
 			xa.rows_pad = p.rows_pad;
