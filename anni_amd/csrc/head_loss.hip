@@ -494,6 +494,33 @@ __global__ __launch_bounds__(kThreads) void head_rows_kernel(RowArgs a)
 		a.bs[v] = v >= a.vocab ? -INFINITY : a.bias ? a.bias[v] : 0.0f;
 }
 
+/* ws[d][ld_ws] = w[d][vocab], zeros up to vocab_pad: lines that are aligned. */
+__global__ __launch_bounds__(kThreads) void head_align_kernel(const uint16_t *w, int d, int vocab, int vocab_pad,
+	uint16_t *ws, int64_t ld_ws)
+{
+	const int per = vocab_pad / 8;
+	const int64_t n = (int64_t)d * per;
+
+	for (int64_t q = (int64_t)blockIdx.x * kThreads + threadIdx.x; q < n; q += (int64_t)gridDim.x * kThreads) {
+		const int64_t r = q / per;
+		const int c = (int)(q - r * per) * 8;
+		u32x4 x = {0u, 0u, 0u, 0u};
+
+		if (c + 8 <= vocab) {
+			x = *(const u32x4_any *)(w + r * vocab + c);
+		} else if (c < vocab) {
+			uint32_t e[4] = {0u, 0u, 0u, 0u};
+
+#pragma unroll
+			for (int j = 0; j < 8; j++)
+				if (c + j < vocab)
+					e[j / 2] |= (uint32_t)w[r * vocab + c + j] << (16 * (j & 1));
+			x = u32x4{e[0], e[1], e[2], e[3]};
+		}
+		*(u32x4 *)(ws + r * ld_ws + c) = x;
+	}
+}
+
 /* ---- logits, by tile: their softmax's running statistics, or delta ----------------------------- */
 
 struct LogitArgs {
@@ -1218,7 +1245,9 @@ struct HeadPlan {
 	int	side_w;		/* of dw's tiles */
 	int	splits_w;	/* slices of the tokens in dw */
 	int64_t	slot_rows_w;
-	size_t	off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_kept, off_slot, off_slot_w;
+	bool	align;		/* w is copied to lines that are aligned */
+	int64_t	ld_ws;
+	size_t	off_ws, off_xs, off_ts, off_bs, off_part, off_hit, off_lse, off_delta, off_kept, off_slot, off_slot_w;
 	bool	keeps;		/* the logits, if there is room */
 	size_t	bytes;		/* the least work area */
 	size_t	bytes_keep;	/* one that holds the logits between the passes */
@@ -1283,6 +1312,24 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	p->tiles_v = count(vocab, p->tile_v);
 	p->parts = grad_type == ANNI_F32 ? 2 : 1;
 	p->ld_xs = p->d_pad + kOdd;
+	/*
+	** Lines that are not aligned go through registers, one step ahead.  That costs a step of the first turn
+	** of tiles about 1.3 us and of a later one .45; a copy of w with aligned lines costs 3 us and .75
+	** for each million of its elements.  Copied where it pays with a third to spare (scoring, us without / with:
+	** 397 x 759 x 1455 32.6 / 20.4, 3000 x 1290 x 4882 96 / 62, 4096 x 712 x 50257 421 / 379, and against it 256 x
+	** 712 x 50257 55 / 65, 500 x 128 x 1001 13 / 17).
+	*/
+	{
+		const int64_t tiles = p->rows_pad / p->tile_t * p->tiles_v;
+		const int64_t turns = count(tiles, p->small ? 2 * kUnits : kUnits);
+
+		p->align = vocab % 8 != 0
+		    && (double)count(d, kStep) * (1.3 + 0.45 * (double)(turns - 1)) > 1.3 * (3.0 + 0.75e-6 * d * vocab);
+	}
+	p->ld_ws = p->vocab_pad + kOdd;
+	p->off_ws = at;
+	if (p->align)
+		at = up(at + (size_t)d * p->ld_ws * 2, 256);
 	p->off_xs = at;
 	at = up(at + (size_t)p->rows_pad * p->ld_xs * 2, 256);
 	p->off_ts = at;
@@ -1511,11 +1558,18 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	hipLaunchKernelGGL(head_rows_kernel, dim3(rows_grid(p.rows_pad * (p.d_pad / 8))), dim3(kThreads), 0, st, ra);
 
 	memset(&la, 0, sizeof(la));
+	if (p.align) {
+		uint16_t *ws = (uint16_t *)(work + p.off_ws);
+
+		hipLaunchKernelGGL(head_align_kernel, dim3(rows_grid(j.d * (p.vocab_pad / 8))), dim3(kThreads), 0, st, w,
+		    j.d, j.vocab, (int)p.vocab_pad, ws, p.ld_ws);
+		w = ws;
+	}
 	la.w.part[0] = la.w.part[1] = w;
-	la.w.ld = (uint32_t)j.vocab;
-	la.w.rows = j.vocab;
+	la.w.ld = (uint32_t)(p.align ? p.ld_ws : j.vocab);
+	la.w.rows = p.align ? p.vocab_pad : j.vocab;
 	la.w.depth = j.d;
-	la.w.aligned = ((uintptr_t)w & 15) == 0 && j.vocab % 8 == 0;
+	la.w.aligned = p.align || (((uintptr_t)w & 15) == 0 && j.vocab % 8 == 0);
 	la.x.part[0] = la.x.part[1] = xs;
 	la.x.ld = (uint32_t)p.ld_xs;
 	la.x.rows = p.rows_pad;
@@ -1605,9 +1659,9 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			xa.delta.rows = p.rows_pad;
 			xa.delta.depth = here;
 			xa.w.part[0] = xa.w.part[1] = w + v0;
-			xa.w.ld = (uint32_t)j.vocab;
+			xa.w.ld = la.w.ld;
 			xa.w.rows = j.d;
-			xa.w.depth = left;
+			xa.w.depth = p.align ? here : left;
 			xa.w.aligned = la.w.aligned;	/* v0 is a multiple of kSide */
 			xa.steps = (int)((left < here ? left : here) + kStep - 1) / kStep;
 			xa.parts = p.parts;

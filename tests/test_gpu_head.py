@@ -151,6 +151,20 @@ def test_many_tokens_and_a_small_vocabulary(gpu, rows, d, vocab, grad_type):
             assert same_bits(got, a if name in parts else b), name
 
 
+@pytest.mark.parametrize("grad_type", [F32, BF16])
+@pytest.mark.parametrize("rows,d,vocab,pad", [(150, 500, 403, 0.2), (1030, 270, 801, 0.0), (700, 520, 1001, 0.5)])
+def test_odd_vocabularies_whose_weights_are_copied(gpu, rows, d, vocab, pad, grad_type):
+    """Sizes at which the lines of w are laid out anew (the work area grows by d lines against an even vocabulary)."""
+    even = gpu.anni_head_loss_work_bytes(rows, d, (vocab + 7) // 8 * 8, grad_type)
+    assert gpu.anni_head_loss_work_bytes(rows, d, vocab, grad_type) >= even + d * vocab * 2
+    c = Case(rows, d, vocab, grad_type, pad=pad, skew=1)
+    c.place()
+    plan = c.plan()
+    plan.work.upload(np.full(plan.work.nbytes, 0xFF, np.uint8))
+    c.run(plan)
+    c.check()
+
+
 @pytest.mark.parametrize("rows,d,vocab", SIZES)
 def test_the_loss_alone_has_the_same_bits(gpu, rows, d, vocab):
     c = Case(rows, d, vocab, F32)
