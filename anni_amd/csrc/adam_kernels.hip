@@ -1183,36 +1183,36 @@ __device__ __forceinline__ void tile_slow(const UpdateArgs &a, const TileInfo &t
 	if constexpr (MT == kQ8) {
 		tile_slow_q8<GT, DER>(a, t, gs, tid, part);
 	} else {
-	for (int64_t i = t.base + tid; i < t.end; i += kThreads) {
-		uint32_t flags = a.uniform_flags;
-		float sc = 1.0f;
+		for (int64_t i = t.base + tid; i < t.end; i += kThreads) {
+			uint32_t flags = a.uniform_flags;
+			float sc = 1.0f;
 
-		if (a.segs) {
-			while (i >= a.segs[s].end)
-				s++;
-			flags = a.segs[s].flags;
+			if (a.segs) {
+				while (i >= a.segs[s].end)
+					s++;
+				flags = a.segs[s].flags;
+			}
+			if (GT == kFP8)
+				sc = a.gscale[s];
+			const Elem e = adam_elem<(GT != kF32 || MT != kF32)>(a.p[i], load_one<GT>(a.g, i, sc),
+			    load_one<MT>(a.m, i, 1.0f), load_one<MT>(a.v, i, 1.0f), gs, a.c,
+			    a.c.decay_on && (flags & kSegDecay) != 0);
+
+			a.p[i] = e.p;
+			store_one<MT>(a.m, i, e.m);
+			store_one<MT>(a.v, i, e.v);
+			zero_one<GT>(a.g, i);
+			if ((flags & kSegTwin) != 0 && a.twin != nullptr)
+				a.twin[i] = (uint16_t)bf16_rne(e.p);
+			if (DER && (flags & kSegFp8Twin) != 0 && a.der.wamax != nullptr) {
+				const float ab = fmaxf(0.0f, fabsf(e.p));
+
+				if (ab > 0.0f)
+					amax_raise(a.der.wamax + s, ab);
+			}
+			if (DER && (flags & kSegPack) != 0 && a.der.pack != nullptr)
+				pack_one(a.der.pack, a.der.packs[s], (uint32_t)(i - a.segs[s].begin), e.p);
 		}
-		if (GT == kFP8)
-			sc = a.gscale[s];
-		const Elem e = adam_elem<(GT != kF32 || MT != kF32)>(a.p[i], load_one<GT>(a.g, i, sc),
-		    load_one<MT>(a.m, i, 1.0f), load_one<MT>(a.v, i, 1.0f), gs, a.c,
-		    a.c.decay_on && (flags & kSegDecay) != 0);
-
-		a.p[i] = e.p;
-		store_one<MT>(a.m, i, e.m);
-		store_one<MT>(a.v, i, e.v);
-		zero_one<GT>(a.g, i);
-		if ((flags & kSegTwin) != 0 && a.twin != nullptr)
-			a.twin[i] = (uint16_t)bf16_rne(e.p);
-		if (DER && (flags & kSegFp8Twin) != 0 && a.der.wamax != nullptr) {
-			const float ab = fmaxf(0.0f, fabsf(e.p));
-
-			if (ab > 0.0f)
-				amax_raise(a.der.wamax + s, ab);
-		}
-		if (DER && (flags & kSegPack) != 0 && a.der.pack != nullptr)
-			pack_one(a.der.pack, a.der.packs[s], (uint32_t)(i - a.segs[s].begin), e.p);
-	}
 	}
 }
 
@@ -2414,20 +2414,20 @@ static void update_launch(hipStream_t st, int grid, const UpdateArgs &a)
 		return;
 	}
 	if constexpr (MT != kQ8) {
-	if (der) {
-		if (nt_on())
-			hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, true, true>), dim3(grid),
+		if (der) {
+			if (nt_on())
+				hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, true, true>), dim3(grid),
+				    dim3(kThreads), 0, st, a);
+			else
+				hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, false, true>), dim3(grid),
+				    dim3(kThreads), 0, st, a);
+		} else if (nt_on()) {
+			hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, true, false>), dim3(grid),
 			    dim3(kThreads), 0, st, a);
-		else
-			hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, false, true>), dim3(grid),
+		} else {
+			hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, false, false>), dim3(grid),
 			    dim3(kThreads), 0, st, a);
-	} else if (nt_on()) {
-		hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, true, false>), dim3(grid),
-		    dim3(kThreads), 0, st, a);
-	} else {
-		hipLaunchKernelGGL((adam_update_kernel<GT, MT, U, false, false>), dim3(grid),
-		    dim3(kThreads), 0, st, a);
-	}
+		}
 	}
 }
 

@@ -1,25 +1,31 @@
 /*
-** Softmax cross entropy of the language model's head over the whole vocabulary, with its gradients,
-** without the logits in memory (include/anni_adam.h, "the head's loss").
+** Softmax cross entropy of the language model's head over the whole vocabulary, with its gradients
+** (include/anni_adam.h, "the head's loss").
 **
 **   logits l[i][v] = sum_d x[i][d] w[d][v] + b[v]
 **   nll[i] = log sum_v exp(l[i][v]) - l[i][target_i]
 **   delta[i][v] = scale (exp(l[i][v] - lse_i) - [v = target_i])
 **   dx = delta w^T,  dw += x^T delta,  db += sum_i delta[i]
 **
-** Four products, two of them the same: the first pass over the vocabulary keeps a running maximum
-** and sum per token and throws the logits away; the second forms them again, a piece of the
-** vocabulary at a time, turns them into delta (bf16, in the work area) and the other two products
-** read it.  Recomputing costs a third more operations than the 6 rows d vocab that cannot be
-** avoided; keeping the logits would cost 4 rows vocab bytes.  With float gradients delta is kept as
-** the sum of two bf16 numbers (16 bits of fraction, an error of 2^-17 against 2^-9), and the two
-** products that read it run over both.
+** The first pass over the vocabulary keeps a maximum and a sum of exponentials per token and tile;
+** scoring ends there, and nothing of the size of the logits is stored.  For gradients the second
+** pass turns logits into delta (bf16, in the work area, a piece of the vocabulary of at most 512 MiB
+** at a time), which the other two products read.  The logits come from the first pass where the work
+** area has room for them, 8 bytes of traffic for each, and are computed again where it has not: a third
+** more operations than the 6 rows d vocab that cannot be avoided (4096 tokens, 1536 x 100000: 1.41 +
+** 0.38 ms against 1.20 + 1.38).  With float gradients delta is the sum of two bf16 numbers (16 bits
+** of fraction, an error of 2^-17 against 2^-9), and the two products that read it run over both.
 **
-** All products are the one kernel below on bf16 operands with float sums: a workgroup of eight
-** wavefronts owns a tile of the result, walks the contracted axis in steps of 64 with the next
-** step's operands on the way into registers, and feeds 32 x 32 x 16 matrix instructions from LDS.
+** The products are one template on bf16 operands with float sums: a workgroup of four or eight
+** wavefronts owns a tile of the result and walks the contracted axis in steps of 64, which go from
+** memory straight into LDS while the step before is multiplied, and feeds 32 x 32 x 16 matrix
+** instructions from there.
 ** An operand lies in memory either with the contracted axis contiguous, or with its rows contiguous;
 ** the second kind is turned by the transposing LDS read, so nothing is transposed in memory.
+**
+** 4096 x 1536 x 100000 in bf16 runs at 1050 TFLOP/s in the first pass, 1090 in dx and 1030 in dw, where the
+** library's product of the same shape reaches 1090 (matrix pipes 69 % busy at 1.66 GHz; here 55 % at
+** 2.05: the chip's power is what either runs into).
 */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -556,7 +562,7 @@ __device__ __forceinline__ f32x4 *kept_block(f32x4 *kept, int64_t kept_v, int64_
 	return kept + ((token / 32) * kept_v + place / 32) * 256;
 }
 
-/* A tile of VOCAB places and TOKENS tokens, or of the model's width and tokens, to a workgroup. */
+/* A tile of SIDE places (or columns of the model's width) and TOKENS tokens to a workgroup. */
 template <int SIDE_, int TOKENS_, int WAVES_, int WAVES_SIDE_, int STAGES_> struct Shape {
 	static constexpr int side = SIDE_;
 	static constexpr int tokens = TOKENS_;
@@ -568,6 +574,7 @@ template <int SIDE_, int TOKENS_, int WAVES_, int WAVES_SIDE_, int STAGES_> stru
 };
 
 /*
+** Tiles of vocabulary by tokens (the logits), of the model's width by tokens (dx).
 ** Many: two stages of the largest tile that fits, one workgroup to a compute unit.  Some: a quarter of
 ** it, two workgroups to a compute unit, where the large tiles would not fill the chip or w is read
 ** more than it is computed with (few rows).  Few: a quarter again, where even those are too few.
@@ -730,7 +737,8 @@ __global__ __launch_bounds__(S::threads) void head_logits_kernel(LogitArgs a)
 					}
 			__syncthreads();
 #pragma unroll
-			for (int c = tid; c < TT * (TV / 8); c += S::threads) {
+			for (int u = 0; u < TT * (TV / 8) / S::threads; u++) {
+				const int c = u * S::threads + tid;
 				const int t = c / (TV / 8);
 				const int chunk = c % (TV / 8);
 
@@ -845,8 +853,9 @@ struct DeltaArgs {
 };
 
 /*
-** 32 tokens by 128 places to a workgroup, a block to a wavefront, turned in LDS into lines of 256
-** bytes.
+** A stream: 4 bytes in and 2 (or 4) out for each.  32 tokens by 128 places to a workgroup, a block to
+** a wavefront, turned in LDS into lines of 256 bytes.  4096 x 50000: 190 us, 6.4 TB/s; two parts,
+** 4096 x 16384: 92 us, 5.8 TB/s.
 */
 template <bool PAIR>
 __global__ __launch_bounds__(kThreads) void head_delta_kernel(DeltaArgs a)
@@ -920,7 +929,11 @@ struct DxArgs {
 	int		add;		/* later pieces of the vocabulary add to the slots */
 };
 
-/* Each slice of the contracted axis (the vocabulary) has a slot of its own. */
+/*
+** Each slice of the contracted axis (the vocabulary) has a slot of its own.  w's lines are the contiguous
+** axis: 128 bytes of each per step.  4096 x 1536 x 50000 570 us, 1100 TFLOP/s; 96 x 1536 x 100000
+** 103 us for w's 307 MB.
+*/
 template <class S>
 __global__ __launch_bounds__(S::threads) void head_dx_kernel(DxArgs a)
 {
@@ -1058,6 +1071,9 @@ __device__ __forceinline__ void add_some(void *base, int64_t i, int64_t n, const
 /*
 ** SIDE: of the tile both ways.  Few tokens leave little to contract and dw to read and write: smaller
 ** tiles then, several workgroups to a compute unit, one at its products while others are at theirs.
+** 96 tokens, 1536 x 100000 bf16: 170 us for 614 MB of dw in and out, 3.6 TB/s; non-temporal accesses and
+** old values read ahead of the products were no faster.  4096 tokens: 610 us for half the
+** vocabulary, 1030 TFLOP/s.
 */
 template <int SIDE, int GT, bool SLICED>
 __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwArgs a)

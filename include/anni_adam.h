@@ -44,11 +44,13 @@ extern "C" {
 **   v  unsigned code, five exponent and three fraction bits: field f > 0: (1 + r / 8) * 2^(E + f - 31),
 **      field 0: r * 2^(E - 33)
 ** d_m and d_v hold ceil(n / 256) * 256 code bytes, then ceil(n / 256) exponent bytes: 2.008 bytes
-** per parameter for both, against 8 with ANNI_F32.  The step computes with the decoded values in
-** double like every other mode, uses the new moments unrounded, and then rounds them to the
+** per parameter for both, against 8 with ANNI_F32.  The step computes the new moments from the
+** decoded ones in double with the host loop's bits, uses them unrounded, and then rounds them to the
 ** formats with a dither: up with the probability of the place between the two neighbours, by a
 ** hash of the element's index and t, so that averages as slow as beta2 = 0.999 still move (to
 ** nearest they would not: a step's change is less than half a code) and runs repeat bit for bit.
+** The step on p is within 2^-43 of the host loop's quotient: the float that p becomes is its neighbour
+** in about one element of 10^8.
 ** A positive v is stored as at least the smallest code.  A block that holds a value that is not
 ** finite reads as NaN as a whole (B = 255); skip_nonfinite keeps such gradients out.  Values below
 ** the smallest float (a block of v whose largest is under 2^-116) lose bits when they are read.
@@ -356,9 +358,9 @@ int	anni_colsum_add_batch(const anni_colsum *jobs, int n_jobs);
 
 /*
 ** The head's loss: softmax cross entropy of logits = x w + b over the whole vocabulary, with its
-** gradients; whole matrices of logits or probabilities need not fit into memory.  x is bf16 [rows][ld_x] (the last hidden states), w the
-** bf16 [d][vocab] matrix the step keeps as the twin of w_head (lang/lm.c's logits = h w_head + b_head), b float [vocab]
-** or NULL.
+** gradients; whole matrices of logits or probabilities need not fit into memory.  x is bf16
+** [rows][ld_x] (the last hidden states), w the bf16 [d][vocab] matrix the step keeps as the twin of
+** w_head (lang/lm.c's logits = h w_head + b_head), b float [vocab] or NULL.
 **   nll[i] = log sum_v exp(l[i][v]) - l[i][target_i]
 **   delta[i][v] = scale * (exp(l[i][v] - lse_i) - [v == target_i])
 **   dx = delta w^T (overwritten),  dw += x^T delta,  db += column sums of delta
@@ -374,10 +376,11 @@ int	anni_colsum_add_batch(const anni_colsum *jobs, int n_jobs);
 **
 ** d_work: work_bytes of device memory, 256-byte aligned, at least anni_head_loss_work_bytes of the
 ** same sizes; nothing is kept in it between calls, and calls on different streams (or recorded
-** into graphs that may run at the same time) need one each.  It holds a copy of x, and for gradients
-** a piece of delta of at most 512 MiB (more only if 256 places of the vocabulary need it), what dx
-** is summed from (float, a copy for each slice of the vocabulary that works on it, up to 64 for small ones), the same for dw where the
-** vocabulary is small, and the logits if there is room.  Nothing else is allocated and nothing waits for the host.
+** into graphs that may run at the same time) need one each.  It holds a copy of x (and of w, where the
+** vocabulary is odd and that pays), and for gradients a piece of delta of at most 512 MiB (more only
+** if 256 places of the vocabulary need it), the slices that dx and dw are summed from (float), and
+** the logits if there is room.  Nothing else is allocated and nothing waits for the host.
+** dw and db must not overlap the inputs; dx may be x.
 */
 typedef struct anni_head_job {
 	int64_t		rows;		/* up to 2^22, and rows * vocab up to 2^38 */
@@ -400,9 +403,9 @@ typedef struct anni_head_job {
 } anni_head_job;
 /*
 ** grad_type -1: the loss alone.  0 for sizes or a type that are refused.  The first is the least; with
-** the second or more the logits of gradients stay in memory between the two passes (4 bytes for each of
-** rows * vocab, padded) instead of being computed again: the same bits sooner.  Up to 512 MiB of logits are part of the
-** first as well.
+** the second or more the logits of gradients stay in memory between the two passes (4 bytes for
+** each of rows * vocab, padded) instead of being computed again: the same bits sooner.  Up to 512
+** MiB of logits are part of the first as well; below a width of 192 the two are the same.
 */
 size_t	anni_head_loss_work_bytes(int64_t rows, int d, int vocab, int grad_type);
 size_t	anni_head_loss_work_bytes_keep(int64_t rows, int d, int vocab, int grad_type);

@@ -299,6 +299,14 @@ def test_logits_kept_or_computed_again_are_the_same_bits(gpu, rows, d, vocab, gr
     assert got[0] == got[1]
 
 
+def test_dx_in_the_place_of_x(gpu):
+    c = Case(130, 72, 520, BF16)
+    c.place()
+    c.ddx = c.dx_
+    c.run(c.plan())
+    c.check()
+
+
 def test_a_freed_plan_is_refused(gpu):
     c = Case(8, 16, 40, F32, model=False)
     c.place()
