@@ -377,7 +377,7 @@ int	anni_colsum_add_batch(const anni_colsum *jobs, int n_jobs);
 ** d_work: work_bytes of device memory, 256-byte aligned, at least anni_head_loss_work_bytes of the
 ** same sizes; nothing is kept in it between calls, and calls on different streams (or recorded
 ** into graphs that may run at the same time) need one each.  It holds a copy of x (and of w, where the
-** vocabulary is odd and that pays), and for gradients a piece of delta of at most 512 MiB (more only
+** vocabulary is no multiple of 8 and that pays), and for gradients a piece of delta of at most 512 MiB (more only
 ** if 256 places of the vocabulary need it), the slices that dx and dw are summed from (float), and
 ** the logits if there is room.  Nothing else is allocated and nothing waits for the host.
 ** dw and db must not overlap the inputs; dx may be x.
