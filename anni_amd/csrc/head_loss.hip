@@ -448,7 +448,7 @@ __device__ __forceinline__ bool tile_of(int64_t id, int64_t tiles_a, int64_t til
 	return true;
 }
 
-/* ---- rows: a clean copy of x and of the targets --------------------------------------------- */
+/* ---- clean copies of x, the targets, the bias, and w's lines --------------------------------------------- */
 
 struct RowArgs {
 	const uint16_t	*x;
@@ -462,12 +462,34 @@ struct RowArgs {
 	int64_t		ld_xs;
 	int32_t		*ts;
 	float		*bs;
+	const uint16_t	*w;
+	uint16_t	*ws;		/* [d][ld_ws], or NULL */
+	int64_t		ld_ws;
 };
+
+/* Eight elements from column c on of a line of n; zeros beyond. */
+__device__ __forceinline__ u32x4 eight_of(const uint16_t *line, int c, int n)
+{
+	u32x4 w = {0u, 0u, 0u, 0u};
+
+	if (c + 8 <= n) {
+		w = *(const u32x4_any *)(line + c);
+	} else if (c < n) {
+		uint32_t e[8];
+
+#pragma unroll
+		for (int j = 0; j < 8; j++)
+			e[j] = c + j < n ? line[c + j] : 0u;
+		w = u32x4{e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16)};
+	}
+	return w;
+}
 
 /*
 ** xs[rows_pad][d_pad] = x, with zeros for rows without a target (whatever x holds there) and beyond
 ** rows and d; ts = target, -1 for rows without one; bs = bias, -inf beyond the vocabulary (which has
-** probability 0 there, and so no delta).  The products then need no masks.
+** probability 0 there, and so no delta).  The products then need no masks.  ws[d][vocab_pad] = w where
+** its lines are to be aligned.
 */
 __global__ __launch_bounds__(kThreads) void head_rows_kernel(RowArgs a)
 {
@@ -479,51 +501,22 @@ __global__ __launch_bounds__(kThreads) void head_rows_kernel(RowArgs a)
 		const int c = (int)(q - r * per) * 8;
 		const int32_t t = r < a.rows ? a.target[r] : -1;
 		const bool live = t >= 0 && t < a.vocab;
-		u32x4 w = {0u, 0u, 0u, 0u};
-
-		if (live && c + 8 <= a.d) {
-			w = *(const u32x4_any *)(a.x + r * a.ld_x + c);
-		} else if (live) {
-			uint32_t e[4] = {0u, 0u, 0u, 0u};
-
-			for (int j = 0; j < 8; j++)
-				if (c + j < a.d)
-					e[j / 2] |= (uint32_t)a.x[r * a.ld_x + c + j] << (16 * (j & 1));
-			w = u32x4{e[0], e[1], e[2], e[3]};
-		}
-		*(u32x4 *)(a.xs + r * a.ld_xs + c) = w;
+		*(u32x4 *)(a.xs + r * a.ld_xs + c) = live ? eight_of(a.x + r * a.ld_x, c, a.d) : u32x4{0u, 0u, 0u, 0u};
 		if (c == 0)
 			a.ts[r] = live ? t : -1;
 	}
 	for (int64_t v = (int64_t)blockIdx.x * kThreads + threadIdx.x; v < a.vocab_pad;
 	    v += (int64_t)gridDim.x * kThreads)
 		a.bs[v] = v >= a.vocab ? -INFINITY : a.bias ? a.bias[v] : 0.0f;
-}
+	if (!a.ws)
+		return;
+	const int64_t per_w = a.vocab_pad / 8;
 
-/* ws[d][ld_ws] = w[d][vocab], zeros up to vocab_pad: lines that are aligned. */
-__global__ __launch_bounds__(kThreads) void head_align_kernel(const uint16_t *w, int d, int vocab, int vocab_pad,
-	uint16_t *ws, int64_t ld_ws)
-{
-	const int per = vocab_pad / 8;
-	const int64_t n = (int64_t)d * per;
+	for (int64_t q = (int64_t)blockIdx.x * kThreads + threadIdx.x; q < a.d * per_w; q += (int64_t)gridDim.x * kThreads) {
+		const int64_t r = q / per_w;
+		const int c = (int)(q - r * per_w) * 8;
 
-	for (int64_t q = (int64_t)blockIdx.x * kThreads + threadIdx.x; q < n; q += (int64_t)gridDim.x * kThreads) {
-		const int64_t r = q / per;
-		const int c = (int)(q - r * per) * 8;
-		u32x4 x = {0u, 0u, 0u, 0u};
-
-		if (c + 8 <= vocab) {
-			x = *(const u32x4_any *)(w + r * vocab + c);
-		} else if (c < vocab) {
-			uint32_t e[4] = {0u, 0u, 0u, 0u};
-
-#pragma unroll
-			for (int j = 0; j < 8; j++)
-				if (c + j < vocab)
-					e[j / 2] |= (uint32_t)w[r * vocab + c + j] << (16 * (j & 1));
-			x = u32x4{e[0], e[1], e[2], e[3]};
-		}
-		*(u32x4 *)(ws + r * ld_ws + c) = x;
+		*(u32x4 *)(a.ws + r * a.ld_ws + c) = eight_of(a.w + r * a.vocab, c, a.vocab);
 	}
 }
 
@@ -1571,16 +1564,17 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	ra.ld_xs = p.ld_xs;
 	ra.ts = ts;
 	ra.bs = (float *)(work + p.off_bs);
-	hipLaunchKernelGGL(head_rows_kernel, dim3(rows_grid(p.rows_pad * (p.d_pad / 8))), dim3(kThreads), 0, st, ra);
+	if (p.align) {
+		ra.w = w;
+		ra.ws = (uint16_t *)(work + p.off_ws);
+		ra.ld_ws = p.ld_ws;
+		w = ra.ws;
+	}
+	const int64_t chunks = p.rows_pad * (p.d_pad / 8), chunks_w = p.align ? j.d * (p.vocab_pad / 8) : 0;
+
+	hipLaunchKernelGGL(head_rows_kernel, dim3(rows_grid(chunks > chunks_w ? chunks : chunks_w)), dim3(kThreads), 0, st, ra);
 
 	memset(&la, 0, sizeof(la));
-	if (p.align) {
-		uint16_t *ws = (uint16_t *)(work + p.off_ws);
-
-		hipLaunchKernelGGL(head_align_kernel, dim3(rows_grid(j.d * (p.vocab_pad / 8))), dim3(kThreads), 0, st, w,
-		    j.d, j.vocab, (int)p.vocab_pad, ws, p.ld_ws);
-		w = ws;
-	}
 	la.w.part[0] = la.w.part[1] = w;
 	la.w.ld = (uint32_t)(p.align ? p.ld_ws : j.vocab);
 	la.w.rows = p.align ? p.vocab_pad : j.vocab;
