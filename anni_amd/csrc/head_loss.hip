@@ -746,6 +746,31 @@ __global__ __launch_bounds__(S::threads) void head_logits_kernel(LogitArgs a)
 
 /* ---- the statistics of all tiles -> lse and nll ------------------------------------------------ */
 
+constexpr int kFewTiles = 32;
+
+/*
+** Few tiles: a lane folds its token's alone, all on their way at once, by their common maximum.  The same
+** function (so the same bits) here and in the pass over kept logits, which then needs no launch ahead of it.
+*/
+__device__ __forceinline__ f32x2 few_stats(const f32x2 *part, int64_t rows_pad, int tiles, int64_t t)
+{
+	f32x2 p[kFewTiles];
+	float top = -INFINITY, sum = 0.0f;
+
+#pragma unroll
+	for (int k = 0; k < kFewTiles; k++)
+		p[k] = k < tiles ? part[k * rows_pad + t] : f32x2{-INFINITY, 0.0f};
+#pragma unroll
+	for (int k = 0; k < kFewTiles; k++)
+		top = fmaxf(top, p[k].x);
+	const float ref = top == -INFINITY ? 0.0f : top;
+
+#pragma unroll
+	for (int k = 0; k < kFewTiles; k++)
+		sum += p[k].y * __expf(p[k].x - ref);
+	return f32x2{top, sum};
+}
+
 struct FinishArgs {
 	const f32x2	*part;
 	const float	*target_logit;
@@ -765,6 +790,19 @@ __device__ __forceinline__ void fold_stats(float &top, float &sum, f32x2 p)
 	top = m;
 }
 
+/* lse of token t, and its nll. */
+__device__ __forceinline__ float put_nll(const FinishArgs &a, int64_t t, f32x2 stats)
+{
+	const float log_sum = logf(stats.y);
+	const float lse = stats.x + log_sum;
+
+	if (a.lse)
+		a.lse[t] = lse;
+	if (t < a.rows)
+		a.nll[t] = a.target[t] >= 0 ? (stats.x - a.target_logit[t]) + log_sum : 0.0f;
+	return lse;
+}
+
 /*
 ** 16 tokens to a workgroup; its groups of 16 lanes, a wavefront of them for every four tiles up to
 ** sixteen wavefronts, share the tiles, eight at a time on their way (782 tiles, 96 tokens: 5.5 us;
@@ -782,6 +820,11 @@ __global__ __launch_bounds__(kFinishWaves * 64) void head_finish_kernel(FinishAr
 	const int64_t t = (int64_t)blockIdx.x * kFinishTokens + token;
 	float top = -INFINITY, sum = 0.0f;
 
+	if (a.tiles_v <= kFewTiles) {
+		if (share == 0)
+			put_nll(a, t, few_stats(a.part, a.rows_pad, (int)a.tiles_v, t));
+		return;
+	}
 	for (int64_t k0 = share; k0 < a.tiles_v; k0 += 8 * parts) {
 		f32x2 p[8];
 		float m = top;
@@ -820,18 +863,14 @@ __global__ __launch_bounds__(kFinishWaves * 64) void head_finish_kernel(FinishAr
 	}
 	if (share != 0)
 		return;
-	const bool live = a.target[t] >= 0;
-	const float log_sum = logf(sum);
-
-	if (a.lse)
-		a.lse[t] = top + log_sum;
-	if (t < a.rows)
-		a.nll[t] = live ? (top - a.target_logit[t]) + log_sum : 0.0f;
+	put_nll(a, t, f32x2{top, sum});
 }
 
 /* ---- delta from logits that were kept ------------------------------------------------------------ */
 
 struct DeltaArgs {
+	FinishArgs	finish;		/* few tiles: the tokens' statistics are folded here */
+	int		few;
 	f32x4		*kept;
 	int64_t		kept_v;
 	const int32_t	*target;
@@ -862,7 +901,6 @@ __global__ __launch_bounds__(kThreads) void head_delta_kernel(DeltaArgs a)
 	const int64_t v_base = a.v0 + c0 + wave * 32;
 	const int t = lane & 31;
 	const int target = a.target[t0 + t];
-	const float lse = a.lse[t0 + t];
 	const int want = target - (int)v_base - block_row(0, lane);
 	/* blocks that lie beyond the vocabulary as a whole may not have been written */
 	const bool inside = v_base < a.vocab;
@@ -873,6 +911,17 @@ __global__ __launch_bounds__(kThreads) void head_delta_kernel(DeltaArgs a)
 #pragma unroll
 	for (int q = 0; q < 4; q++)
 		x[q] = __builtin_nontemporal_load(block + q * 64);
+	float lse;
+
+	if (a.few) {
+		const f32x2 stats = few_stats(a.finish.part, a.finish.rows_pad, a.few, t0 + t);
+
+		lse = stats.x + logf(stats.y);
+		if (c0 == 0 && a.v0 == 0 && tid < 32)
+			put_nll(a.finish, t0 + t, stats);
+	} else {
+		lse = a.lse[t0 + t];
+	}
 #pragma unroll
 	for (int q = 0; q < 4; q++) {
 		const int chunk = (wave * 4 + q) ^ (t & 15);
@@ -984,34 +1033,6 @@ struct DxSumArgs {
 	void		*dx;
 	int64_t		ld_dx;
 };
-
-/* dx = the slots' sum in order, in the caller's type. */
-template <int GT>
-__global__ __launch_bounds__(kThreads) void head_dx_sum_kernel(DxSumArgs a)
-{
-	const int64_t per = a.d_pad / 4;
-	const int64_t n = a.rows * per;
-
-	for (int64_t q = (int64_t)blockIdx.x * kThreads + threadIdx.x; q < n; q += (int64_t)gridDim.x * kThreads) {
-		const int64_t r = q / per;
-		const int c = (int)(q - r * per) * 4;
-		f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-
-		if (c >= a.d)
-			continue;
-#pragma unroll 8
-		for (int k = 0; k < a.splits; k++)
-			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_pad + c);
-#pragma unroll
-		for (int j = 0; j < 4; j++)
-			if (c + j < a.d) {
-				if constexpr (GT == kF32)
-					((float *)a.dx)[r * a.ld_dx + c + j] = s[j];
-				else
-					((uint16_t *)a.dx)[r * a.ld_dx + c + j] = (uint16_t)bf16_rne(s[j]);
-			}
-	}
-}
 
 /* ---- dw and db --------------------------------------------------------------------------------- */
 
@@ -1204,15 +1225,44 @@ struct DwSumArgs {
 	void		*db;
 };
 
-/* dw and db += the slots' sums in order: a line of dw (or db, the last) to a row of workgroups. */
+/* dx = the slots' sum in order, in the caller's type. */
 template <int GT>
-__global__ __launch_bounds__(kThreads) void head_dw_sum_kernel(DwSumArgs a)
+__device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_t blocks)
 {
-	const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+	const int64_t per = a.d_pad / 4;
+	const int64_t n = a.rows * per;
+
+	for (int64_t q = block * kThreads + threadIdx.x; q < n; q += blocks * kThreads) {
+		const int64_t r = q / per;
+		const int c = (int)(q - r * per) * 4;
+		f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+
+		if (c >= a.d)
+			continue;
+#pragma unroll 8
+		for (int k = 0; k < a.splits; k++)
+			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_pad + c);
+#pragma unroll
+		for (int j = 0; j < 4; j++)
+			if (c + j < a.d) {
+				if constexpr (GT == kF32)
+					((float *)a.dx)[r * a.ld_dx + c + j] = s[j];
+				else
+					((uint16_t *)a.dx)[r * a.ld_dx + c + j] = (uint16_t)bf16_rne(s[j]);
+			}
+	}
+}
+
+/* dw and db += the slots' sums in order: a line of dw (or db, the last) to a row of `across` workgroups. */
+template <int GT>
+__device__ __forceinline__ void dw_sum(const DwSumArgs &a, int64_t block, int64_t blocks)
+{
+	const int64_t across = (a.count + kThreads - 1) / kThreads;
+	const int64_t c = block % across * kThreads + threadIdx.x;
 
 	if (c >= a.count)
 		return;
-	for (int64_t r = blockIdx.y; r <= a.d; r += gridDim.y) {
+	for (int64_t r = block / across; r <= a.d; r += blocks / across) {
 		const bool last = r == a.d;
 		const float *p = a.slot + (last ? a.slot_rows : r) * a.ld_slot + c;
 		float s = 0.0f;
@@ -1224,6 +1274,16 @@ __global__ __launch_bounds__(kThreads) void head_dw_sum_kernel(DwSumArgs a)
 			s += p[(int64_t)k * (a.slot_rows + 1) * a.ld_slot];
 		add_to<GT>(last ? a.db : a.dw, last ? a.v0 + c : r * a.vocab + a.v0 + c, s);
 	}
+}
+
+/* Both in one launch: the first blocks_x workgroups are dx's, the others (a multiple of dw_sum's `across`) dw's. */
+template <int GT>
+__global__ __launch_bounds__(kThreads) void head_sums_kernel(DxSumArgs x, unsigned blocks_x, DwSumArgs w)
+{
+	if (blockIdx.x < blocks_x)
+		dx_sum<GT>(x, blockIdx.x, blocks_x);
+	else
+		dw_sum<GT>(w, blockIdx.x - blocks_x, gridDim.x - blocks_x);
 }
 
 /* ---- plan -------------------------------------------------------------------------------------- */
@@ -1465,11 +1525,14 @@ static void logits_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &a)
 }
 
 /* The same from the logits that were kept, for `here` places (a multiple of kSide) of the piece. */
-static void delta_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &l, int64_t here, int vocab)
+static void delta_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &l, const FinishArgs &f, int few, int64_t here,
+	int vocab)
 {
 	DeltaArgs a;
 
 	memset(&a, 0, sizeof(a));
+	a.finish = f;
+	a.few = few;
 	a.kept = l.kept;
 	a.kept_v = l.kept_v;
 	a.target = l.target;
@@ -1517,23 +1580,29 @@ static void dw_launch(hipStream_t st, const HeadPlan &p, const DwArgs &a)
 		hipLaunchKernelGGL((head_dw_kernel<128, GT, false>), grid, dim3(256), 0, st, a);
 	else
 		hipLaunchKernelGGL((head_dw_kernel<256, GT, false>), grid, dim3(512), 0, st, a);
-	if (a.splits > 1) {
-		DwSumArgs s;
+}
 
-		memset(&s, 0, sizeof(s));
-		s.slot = a.slot;
-		s.splits = a.splits;
-		s.slot_rows = a.slot_rows;
-		s.ld_slot = a.ld_slot;
-		s.d = a.d;
-		s.vocab = a.vocab;
-		s.v0 = a.v0;
-		s.count = a.vocab - a.v0 < p.piece ? a.vocab - a.v0 : p.piece;
-		s.dw = a.dw;
-		s.db = a.db;
-		hipLaunchKernelGGL(head_dw_sum_kernel<GT>, dim3((unsigned)count(s.count, kThreads),
-		    (unsigned)(a.d + 1 < 1024 ? a.d + 1 : 1024)), dim3(kThreads), 0, st, s);
+/* x and w: may be NULL */
+static void sums_launch(hipStream_t st, int grad_type, const DxSumArgs *x, const DwSumArgs *w)
+{
+	DxSumArgs ax;
+	DwSumArgs aw;
+	unsigned blocks_x = 0, blocks_w = 0;
+
+	memset(&ax, 0, sizeof(ax));
+	memset(&aw, 0, sizeof(aw));
+	if (x) {
+		ax = *x;
+		blocks_x = (unsigned)rows_grid(x->rows * (x->d_pad / 4));
 	}
+	if (w) {
+		aw = *w;
+		blocks_w = (unsigned)(count(w->count, kThreads) * (w->d + 1 < 1024 ? w->d + 1 : 1024));
+	}
+	if (grad_type == ANNI_F32)
+		hipLaunchKernelGGL(head_sums_kernel<kF32>, dim3(blocks_x + blocks_w), dim3(kThreads), 0, st, ax, blocks_x, aw);
+	else
+		hipLaunchKernelGGL(head_sums_kernel<kBF16>, dim3(blocks_x + blocks_w), dim3(kThreads), 0, st, ax, blocks_x, aw);
 }
 
 static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
@@ -1608,8 +1677,13 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 	fa.rows_pad = p.rows_pad;
 	fa.lse = lse;
 	fa.nll = j.d_nll;
-	hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.rows_pad / kFinishTokens)),
-	    dim3(p.tiles_v < 4 * kFinishWaves ? (unsigned)up((size_t)p.tiles_v, 4) * 16 : kFinishWaves * 64), 0, st, fa);
+	/* nothing but the pass over the kept logits asks for them: it folds them itself */
+	const int few = keep && p.tiles_v <= kFewTiles ? (int)p.tiles_v : 0;
+
+	if (!few)
+		hipLaunchKernelGGL(head_finish_kernel, dim3((unsigned)(p.rows_pad / kFinishTokens)),
+		    dim3(p.tiles_v <= kFewTiles ? 64u : p.tiles_v < 4 * kFinishWaves ? (unsigned)up((size_t)p.tiles_v, 4) * 16
+		    : kFinishWaves * 64), 0, st, fa);
 
 	for (int64_t v0 = 0; grad && v0 < j.vocab; v0 += p.piece) {
 		const int64_t left = j.vocab - v0;
@@ -1618,6 +1692,8 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		uint16_t *low = delta + p.rows_pad * p.ld_delta;
 		DxArgs xa;
 		DwArgs wa;
+		DxSumArgs sx;
+		DwSumArgs sw;
 
 		la.v0 = v0;
 		la.tiles_v = here / p.tile_v;
@@ -1627,7 +1703,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		la.delta_low = low;
 		la.ld_delta = p.ld_delta;
 		if (keep)
-			delta_launch(st, p, la, here, j.vocab);
+			delta_launch(st, p, la, fa, few, here, j.vocab);
 		else if (p.parts == 2)
 			logits_launch<kDeltaPair>(st, p, la);
 		else
@@ -1684,25 +1760,36 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			xa.add = v0 > 0;
 			dx_launch(st, p, xa);
 		}
-	}
-	if (grad && j.d_dx) {
-		DxSumArgs sa;
+		/* the slices' sums: dw's behind every piece, dx's behind the last one */
+		const bool sum_w = wa.splits > 1 && (j.d_dw || j.d_db);
+		const bool sum_x = j.d_dx && left <= p.piece;
 
-		memset(&sa, 0, sizeof(sa));
-		sa.slot = (const float *)(work + p.off_slot);
-		sa.splits = p.splits;
-		sa.rows = j.rows;
-		sa.rows_pad = p.rows_pad;
-		sa.d = j.d;
-		sa.d_pad = p.d_pad;
-		sa.dx = j.d_dx;
-		sa.ld_dx = j.ld_dx;
-		const dim3 grid((unsigned)rows_grid(j.rows * (p.d_pad / 4)));
-
-		if (j.grad_type == ANNI_F32)
-			hipLaunchKernelGGL(head_dx_sum_kernel<kF32>, grid, dim3(kThreads), 0, st, sa);
-		else
-			hipLaunchKernelGGL(head_dx_sum_kernel<kBF16>, grid, dim3(kThreads), 0, st, sa);
+		if (sum_w) {
+			memset(&sw, 0, sizeof(sw));
+			sw.slot = wa.slot;
+			sw.splits = wa.splits;
+			sw.slot_rows = wa.slot_rows;
+			sw.ld_slot = wa.ld_slot;
+			sw.d = j.d;
+			sw.vocab = j.vocab;
+			sw.v0 = v0;
+			sw.count = left < p.piece ? left : p.piece;
+			sw.dw = j.d_dw;
+			sw.db = j.d_db;
+		}
+		if (sum_x) {
+			memset(&sx, 0, sizeof(sx));
+			sx.slot = xa.slot;
+			sx.splits = p.splits;
+			sx.rows = j.rows;
+			sx.rows_pad = p.rows_pad;
+			sx.d = j.d;
+			sx.d_pad = p.d_pad;
+			sx.dx = j.d_dx;
+			sx.ld_dx = j.ld_dx;
+		}
+		if (sum_w || sum_x)
+			sums_launch(st, j.grad_type, sum_x ? &sx : nullptr, sum_w ? &sw : nullptr);
 	}
 	return hip_ok(hipGetLastError(), "head_loss") ? 0 : -1;
 }
