@@ -965,9 +965,9 @@ struct DxArgs {
 	Source		w;
 	int		steps, parts, splits;
 	int64_t		tiles_t, tiles_d;
-	float		*slot;		/* [splits][rows_pad][d_pad] */
+	float		*slot;		/* [splits][rows_pad][d_slot] */
 	int64_t		rows_pad;
-	int		d_pad;
+	int		d_slot;
 	int		add;		/* later pieces of the vocabulary add to the slots */
 };
 
@@ -1008,20 +1008,20 @@ __global__ __launch_bounds__(S::threads) void head_dx_kernel(DxArgs a)
 		for (int j = 0; j < NB; j++) {
 			const int64_t t = tt * TT + wm * (MB * 32) + i * 32 + block_row(0, lane);
 			const int64_t c = td * TD + wn * (NB * 32) + j * 32 + (lane & 31);
-			float *p = a.slot + ((int64_t)slice * a.rows_pad + t) * a.d_pad + c;
+			float *p = a.slot + ((int64_t)slice * a.rows_pad + t) * a.d_slot + c;
 			float old[16];
 
 			if (a.add) {
 #pragma unroll
 				for (int r = 0; r < 16; r++)
-					old[r] = p[(int64_t)block_row(r, 0) * a.d_pad];
+					old[r] = p[(int64_t)block_row(r, 0) * a.d_slot];
 #pragma unroll
 				for (int r = 0; r < 16; r++)
 					acc[i][j][r] += old[r];
 			}
 #pragma unroll
 			for (int r = 0; r < 16; r++)
-				p[(int64_t)block_row(r, 0) * a.d_pad] = acc[i][j][r];
+				p[(int64_t)block_row(r, 0) * a.d_slot] = acc[i][j][r];
 		}
 }
 
@@ -1029,7 +1029,7 @@ struct DxSumArgs {
 	const float	*slot;
 	int		splits;
 	int64_t		rows, rows_pad;
-	int		d, d_pad;
+	int		d, d_slot;
 	void		*dx;
 	int64_t		ld_dx;
 };
@@ -1229,7 +1229,7 @@ struct DwSumArgs {
 template <int GT>
 __device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_t blocks)
 {
-	const int64_t per = a.d_pad / 4;
+	const int64_t per = a.d_slot / 4;
 	const int64_t n = a.rows * per;
 
 	for (int64_t q = block * kThreads + threadIdx.x; q < n; q += blocks * kThreads) {
@@ -1241,7 +1241,7 @@ __device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_
 			continue;
 #pragma unroll 8
 		for (int k = 0; k < a.splits; k++)
-			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_pad + c);
+			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_slot + c);
 #pragma unroll
 		for (int j = 0; j < 4; j++)
 			if (c + j < a.d) {
@@ -1303,6 +1303,7 @@ struct HeadPlan {
 	int	tile_v;		/* the other side of the logits' tiles */
 	int	dx;		/* kDxFew .. kDxMany */
 	int	dx_t, tile_d;	/* its tiles */
+	int	d_slot;		/* columns of a slot: whole tiles */
 	int64_t	rows_pad;
 	int	d_pad;
 	int64_t	vocab_pad;
@@ -1377,6 +1378,7 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 	p->tile_d = p->dx == kDxFew ? DxFew::side : p->dx == kDxMany ? DxMany::side : DxSome::side;
 	p->rows_pad = (int64_t)up((size_t)rows, (size_t)p->tile_t);
 	p->d_pad = (int)up((size_t)d, kSide);
+	p->d_slot = (int)up((size_t)d, (size_t)p->tile_d);
 	p->vocab_pad = (int64_t)up((size_t)vocab, kSide);
 	p->tiles_v = count(vocab, p->tile_v);
 	p->parts = grad_type == ANNI_F32 ? 2 : 1;
@@ -1430,7 +1432,7 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		** 254 x 64 x 256 9.7 / 4.8, 100 x 256 x 2001 18 / 7, 700 x 300 x 2000 17.5 / 11.3).
 		*/
 		const size_t near_slots = (size_t)8 << 20;
-		const size_t slot = (size_t)p->rows_pad * (size_t)p->d_pad * 4;
+		const size_t slot = (size_t)p->rows_pad * (size_t)p->d_slot * 4;
 		const int64_t units = p->dx == kDxMany ? kUnits : 2 * kUnits;	/* few tokens are bound by memory: more on its way */
 
 		p->splits = 1;
@@ -1470,7 +1472,7 @@ static bool head_plan(int64_t rows, int d, int vocab, int grad_type, HeadPlan *p
 		p->off_delta = at;
 		at = up(at + (size_t)p->rows_pad * p->ld_delta * 2 * p->parts, 256);
 		p->off_slot = at;
-		at = up(at + (size_t)p->splits * p->rows_pad * p->d_pad * 4, 256);
+		at = up(at + (size_t)p->splits * p->rows_pad * p->d_slot * 4, 256);
 		p->off_slot_w = at;
 		if (p->splits_w > 1)
 			at = up(at + (size_t)p->splits_w * (p->slot_rows_w + 1) * p->piece * 4, 256);
@@ -1593,7 +1595,7 @@ static void sums_launch(hipStream_t st, int grad_type, const DxSumArgs *x, const
 	memset(&aw, 0, sizeof(aw));
 	if (x) {
 		ax = *x;
-		blocks_x = (unsigned)rows_grid(x->rows * (x->d_pad / 4));
+		blocks_x = (unsigned)rows_grid(x->rows * (x->d_slot / 4));
 	}
 	if (w) {
 		aw = *w;
@@ -1756,7 +1758,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			xa.tiles_d = count(j.d, p.tile_d);	/* every tile has a valid row of w */
 			xa.slot = (float *)(work + p.off_slot);
 			xa.rows_pad = p.rows_pad;
-			xa.d_pad = p.d_pad;
+			xa.d_slot = p.d_slot;
 			xa.add = v0 > 0;
 			dx_launch(st, p, xa);
 		}
@@ -1784,7 +1786,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			sx.rows = j.rows;
 			sx.rows_pad = p.rows_pad;
 			sx.d = j.d;
-			sx.d_pad = p.d_pad;
+			sx.d_slot = p.d_slot;
 			sx.dx = j.d_dx;
 			sx.ld_dx = j.ld_dx;
 		}
