@@ -457,4 +457,6 @@ def test_refusals_on_an_arena(gpu):
         HeadLoss(rows, d, vocab, FP8)
     with pytest.raises(ValueError):
         HeadLoss(rows, d, vocab, F32, grad=False).run(x.ptr, x.ptr, None, t.ptr, nll.ptr, dx=x.ptr)
+    with pytest.raises(ValueError):
+        HeadLoss(rows, d, vocab, F32, grad=False).run_on(None, 0, 1, x.ptr, t.ptr, nll.ptr, dx=x.ptr)
     assert lib.load().anni_head_loss_work_bytes(rows, d, vocab, F32) == plan.work.nbytes
