@@ -299,6 +299,30 @@ def test_logits_kept_or_computed_again_are_the_same_bits(gpu, rows, d, vocab, gr
     assert got[0] == got[1]
 
 
+def test_more_logits_than_32_bits_count(gpu):
+    """36000 x 60160 = 2.17e9 logits, kept and computed again: the same bits; some rows against 64 bits
+    (with bf16 gradients: the bounds of one rounding of delta and of dx, as everywhere)."""
+    from anni_amd.head_loss import HeadLoss
+    rows, d, vocab = 36000, 200, 60160
+    some = np.array([0, 1, 17999, 35712, 35713, 35999])
+    got = []
+    for keep in (True, False):
+        c = Case(rows, d, vocab, BF16, pad=0.1, model=False)
+        c.place()
+        plan = HeadLoss(rows, d, vocab, BF16, keep=keep)
+        c.run(plan)
+        got.append(c.outputs())
+        plan.free()
+        assert all((a == b).all() for a, b in zip(got[0], got[-1]))
+        for b in (c.dx_, c.dww, c.dbias, c.dt, c.dnll, c.ddx, c.ddw, c.ddb):
+            b.buf.free()
+    w = Loss(widen(c.x[some]), widen(c.w), c.b, c.target[some].astype(np.int64), c.scale)
+    nll, dx = got[0][0][some].astype(np.float64), value(got[0][1][some])
+    assert w.live.sum() > 1
+    assert (np.abs(nll - w.nll) <= w.tol_nll).all()
+    assert (np.abs(dx - w.dx) <= w.tolerances(BF16)[0]).all()
+
+
 def test_dx_in_the_place_of_x(gpu):
     c = Case(130, 72, 520, BF16)
     c.place()
