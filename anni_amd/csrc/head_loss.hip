@@ -1082,6 +1082,18 @@ __device__ __forceinline__ void add_some(void *base, int64_t i, int64_t n, const
 		}
 }
 
+/* Sixteen bytes without their first `halves` 16-bit halves, the others in their place. */
+__device__ __forceinline__ u32x4 moved_down(u32x4 w, int halves)
+{
+	if (halves & 4)
+		w = u32x4{w.z, w.w, 0u, 0u};
+	if (halves & 2)
+		w = u32x4{w.y, w.z, w.w, 0u};
+	if (halves & 1)
+		w = u32x4{(w.x >> 16) | (w.y << 16), (w.y >> 16) | (w.z << 16), (w.z >> 16) | (w.w << 16), w.w >> 16};
+	return w;
+}
+
 /*
 ** SIDE: of the tile both ways.  Few tokens leave little to contract and dw to read and write: smaller
 ** tiles then, several workgroups to a compute unit, one at its products while others are at theirs.
@@ -1148,15 +1160,83 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 	/*
 	** The tile through LDS, half its rows at a time, so that dw is read and written in whole lines (a
 	** lane holds one column: two bytes of a line with bf16 gradients, and 96 tokens of the 555M head,
-	** where this is most of the work, took 620 us).
+	** where this is most of the work, took 620 us).  A lane's chunks lie below each other; one that the
+	** vocabulary ends in is read as the line's last sixteen bytes and moved down.
 	*/
 	constexpr int kWide = GT == kF32 ? 4 : 8;		/* elements in sixteen bytes */
 	constexpr int kHalf = SIDE / 2;
-	constexpr int kChunksOf = kHalf * SIDE / kWide / kThreadsHere;	/* of a lane, per half */
+	constexpr int kAcross = SIDE / kWide;			/* chunks to a line */
+	constexpr int kApart = kThreadsHere / kAcross;		/* lines between two chunks of a lane */
+	constexpr int kChunksOf = kHalf / kApart;		/* of a lane, per half */
 	constexpr int kAhead = kChunksOf < 8 ? kChunksOf : 8;	/* of them on their way together */
-	static_assert(kHalf * SIDE / kWide % (kAhead * kThreadsHere) == 0, "whole rounds");
+	static_assert(kThreadsHere % kAcross == 0 && kChunksOf % kAhead == 0, "whole rounds");
 	float *const tile = (float *)lds;			/* [kHalf][SIDE] */
+	const int64_t v = a.v0 + tv * SIDE + tid % kAcross * kWide;
+	const int64_t left = a.vocab - v;			/* elements from the lane's first on */
+	const bool near = a.vocab >= kWide;			/* a line has sixteen bytes */
+	const int beyond = left >= kWide ? 0 : left > 0 ? kWide - (int)left : kWide;
+	char *const first = (char *)a.dw + (v - beyond) * (16 / kWide);
 
+	auto line_of = [&](int h, int u) {
+		const int row = tid / kAcross + u * kApart;
+
+		return td * SIDE + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
+	};
+	auto fetch = [&](int h, int u0, u32x4 (&old)[kAhead]) {
+#pragma unroll
+		for (int u = 0; u < kAhead; u++) {
+			const int64_t k = line_of(h, u0 + u);
+
+			if (k < a.d && beyond < kWide && near)
+				old[u] = *(const u32x4_any *)(first + k * a.vocab * (16 / kWide));
+		}
+	};
+	auto put = [&](int h, int u0, const u32x4 (&old)[kAhead]) {
+#pragma unroll
+		for (int u = 0; u < kAhead; u++) {
+			const int64_t k = line_of(h, u0 + u);
+			const float *x = tile + (tid / kAcross + (u0 + u) * kApart) * SIDE + tid % kAcross * kWide;
+			u32x4 w = old[u];
+
+			if (k >= a.d || beyond == kWide)
+				continue;
+			if (!near) {
+				add_some<GT, kWide>(a.dw, k * a.vocab + v, left, x);
+				continue;
+			}
+			if (beyond)
+				w = moved_down(w, beyond * (8 / kWide));
+			if constexpr (GT == kF32) {
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					w[e] = __float_as_uint(__uint_as_float(w[e]) + x[e]);
+			} else {
+#pragma unroll
+				for (int e = 0; e < 4; e++)
+					w[e] = bf16_rne2(__uint_as_float(w[e] << 16) + x[2 * e],
+					    __uint_as_float(w[e] & 0xffff0000u) + x[2 * e + 1]);
+			}
+			if (beyond == 0) {
+				*(u32x4_any *)(first + k * a.vocab * (16 / kWide)) = w;
+				continue;
+			}
+#pragma unroll
+			for (int e = 0; e < kWide; e++)
+				if (e < left) {
+					if constexpr (GT == kF32)
+						((uint32_t *)a.dw)[k * a.vocab + v + e] = w[e];
+					else
+						((uint16_t *)a.dw)[k * a.vocab + v + e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+				}
+		}
+	};
+	u32x4 old[2][kAhead];
+
+	/* where a half is one round, the second half's old values come with the first's */
+	if constexpr (kChunksOf == kAhead) {
+		fetch(0, 0, old[0]);
+		fetch(1, 0, old[1]);
+	}
 #pragma unroll
 	for (int h = 0; h < 2; h++) {
 		if (h)
@@ -1170,46 +1250,13 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 					tile[(wm * (kHalf / 2) + i * 32 + block_row(r, lane)) * SIDE + wn * (NB * 32) + j * 32
 					    + (lane & 31)] = acc[h * (MB / 2) + i][j][r];
 		__syncthreads();
-		for (int c0 = tid; c0 < kHalf * SIDE / kWide; c0 += kAhead * kThreadsHere) {
-			u32x4 old[kAhead];
-
-#pragma unroll
-			for (int u = 0; u < kAhead; u++) {
-				const int c = c0 + u * kThreadsHere;
-				const int row = c / (SIDE / kWide);
-				const int64_t k = td * SIDE + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
-				const int64_t v = a.v0 + tv * SIDE + c % (SIDE / kWide) * kWide;
-
-				if (k < a.d && v + kWide <= a.vocab)
-					old[u] = *(const u32x4_any *)((const char *)a.dw + (k * a.vocab + v) * (16 / kWide));
-			}
-#pragma unroll
-			for (int u = 0; u < kAhead; u++) {
-				const int c = c0 + u * kThreadsHere;
-				const int row = c / (SIDE / kWide);
-				const int64_t k = td * SIDE + (row / (kHalf / 2)) * kHalf + h * (kHalf / 2) + row % (kHalf / 2);
-				const int64_t v = a.v0 + tv * SIDE + c % (SIDE / kWide) * kWide;
-				const float *x = tile + row * SIDE + c % (SIDE / kWide) * kWide;
-
-				if (k >= a.d)
-					continue;
-				if (v + kWide <= a.vocab) {
-					u32x4 w;
-
-					if constexpr (GT == kF32) {
-#pragma unroll
-						for (int e = 0; e < 4; e++)
-							w[e] = __float_as_uint(__uint_as_float(old[u][e]) + x[e]);
-					} else {
-#pragma unroll
-						for (int e = 0; e < 4; e++)
-							w[e] = bf16_rne2(__uint_as_float(old[u][e] << 16) + x[2 * e],
-							    __uint_as_float(old[u][e] & 0xffff0000u) + x[2 * e + 1]);
-					}
-					*(u32x4_any *)((char *)a.dw + (k * a.vocab + v) * (16 / kWide)) = w;
-				} else {
-					add_some<GT, kWide>(a.dw, k * a.vocab + v, a.vocab - v, x);
-				}
+		if constexpr (kChunksOf == kAhead) {
+			put(h, 0, old[h]);
+		} else {
+#pragma unroll 1
+			for (int u0 = 0; u0 < kChunksOf; u0 += kAhead) {
+				fetch(h, u0, old[0]);
+				put(h, u0, old[0]);
 			}
 		}
 	}
