@@ -397,12 +397,13 @@ typedef struct anni_head_job {
 	int64_t		ld_dx;		/* >= d */
 	void		*d_dw;
 	void		*d_db;
-	int		grad_type;	/* ANNI_F32 or ANNI_BF16, of dx, dw and db */
+	int		grad_type;	/* ANNI_F32 or ANNI_BF16, of dx, dw and db; not read for the loss alone */
 	void		*d_work;
 	size_t		work_bytes;
 } anni_head_job;
 /*
-** grad_type -1: the loss alone.  0 for sizes or a type that are refused.  The first is the least; with
+** grad_type -1 (here only: a job that names it beside gradients is refused): the loss alone.  0 for sizes
+** or a type that are refused.  The first is the least; with
 ** the second or more the logits of gradients stay in memory between the two passes (4 bytes for
 ** each of rows * vocab, padded) instead of being computed again: the same bits sooner.  Up to 512
 ** MiB of logits are part of the first as well; below a width of 192 the two are the same.
