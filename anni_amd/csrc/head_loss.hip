@@ -1003,6 +1003,7 @@ struct DxSumArgs {
 	int		splits;
 	int64_t		rows, rows_pad;
 	int		d, d_slot;
+	const int32_t	*target;	/* ts */
 	void		*dx;
 	int64_t		ld_dx;
 };
@@ -1245,7 +1246,10 @@ struct DwSumArgs {
 	void		*db;
 };
 
-/* dx = the slots' sum in order, in the caller's type. */
+/*
+** dx = the slots' sum in order, in the caller's type.  A row without a target has delta 0, but its product
+** with a w that is not finite is NaN: it gets its 0 here, and its slots are not read.
+*/
 template <int GT>
 __device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_t blocks)
 {
@@ -1259,8 +1263,10 @@ __device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_
 
 		if (c >= a.d)
 			continue;
+		const int splits = a.target[r] >= 0 ? a.splits : 0;
+
 #pragma unroll 8
-		for (int k = 0; k < a.splits; k++)
+		for (int k = 0; k < splits; k++)
 			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_slot + c);
 #pragma unroll
 		for (int j = 0; j < 4; j++)
@@ -1598,6 +1604,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			sx.rows_pad = p.rows_pad;
 			sx.d = j.d;
 			sx.d_slot = p.d_slot;
+			sx.target = ts;
 			sx.dx = j.d_dx;
 			sx.ld_dx = j.ld_dx;
 		}
