@@ -74,16 +74,21 @@ struct Source {
 ** Sixteen bytes per lane from base + offset to 16 l behind `lds` (both uniform but the offset).  In
 ** assembly because behind the builtin the compiler waits for every such load before any read of LDS,
 ** and this one's whole point is to stay on its way; arrived() is the wait, before the barrier that
-** hands the data over.  It writes no register, and loads of the compiler's own only ever wait for more
-** than they must (they return in order).  m0 must have been written one instruction before its use.
+** hands the data over.  It writes no vector register, and loads of the compiler's own only ever wait for
+** more than they must (they return in order).  m0 must have been written one instruction before its use;
+** the clobber tells the compiler that a value of its own there is gone (its warning that the register is a
+** reserved one says that it keeps none across statements anyway: the code is the same).
 */
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void memory_to_lds(const uint16_t *base, uint32_t offset, char *lds)
 {
 	const uint32_t at = (uint32_t)(uintptr_t)(ANNI_LDS char *)lds;
 
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-	    : : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(base) : "memory");
+	    : : "s"(__builtin_amdgcn_readfirstlane(at)), "v"(offset), "s"(base) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 /* All but the LATER last loads have arrived. */
 template <int LATER>
