@@ -4,8 +4,12 @@
 **
 **   logits l[i][v] = sum_d x[i][d] w[d][v] + b[v]
 **   nll[i] = log sum_v exp(l[i][v]) - l[i][target_i]
-**   delta[i][v] = scale (exp(l[i][v] - lse_i) - [v = target_i])
-**   dx = delta w^T,  dw += x^T delta,  db += sum_i delta[i]
+**   delta[i][v] = exp(l[i][v] - lse_i) - [v = target_i]
+**   dx = scale delta w^T,  dw += scale x^T delta,  db += scale sum_i delta[i]
+**
+** scale is a factor of the float sums and no part of delta, which is rounded: nearly all of a loss' delta is -1 at
+** the targets, a number of few bits, and a scale in it (a mean's 1 / rows) would be rounded alike in all of them, an
+** error of up to 2^-8 that no sum averages out (96 tokens, db in bf16: 0.5 % off the formula's, 0.2 without).
 **
 ** The first pass over the vocabulary keeps a maximum and a sum of exponentials per token and tile;
 ** scoring ends there, and nothing of the size of the logits is stored.  For gradients the second
@@ -540,7 +544,6 @@ struct LogitArgs {
 	int64_t		kept_v;		/* blocks along the vocabulary */
 	/* delta */
 	const float	*lse;
-	float		scale;
 	int64_t		v0;		/* first vocabulary place of this piece */
 	uint16_t	*delta;		/* [rows_pad][ld_delta], low halves behind the high ones */
 	uint16_t	*delta_low;
@@ -673,7 +676,7 @@ __global__ __launch_bounds__(S::threads) void head_logits_kernel(LogitArgs a)
 
 					if (want == i * 32 + block_row(r, 0))
 						p -= 1.0f;
-					acc[i][j][r] = live ? p * a.scale : 0.0f;
+					acc[i][j][r] = live ? p : 0.0f;
 				}
 		}
 		/*
@@ -853,7 +856,6 @@ struct DeltaArgs {
 	int64_t		kept_v;
 	const int32_t	*target;
 	const float	*lse;
-	float		scale;
 	int		vocab;
 	int64_t		v0;		/* of this piece */
 	int64_t		groups_v;	/* of 128 places, in this piece */
@@ -911,7 +913,7 @@ __global__ __launch_bounds__(kThreads) void head_delta_kernel(DeltaArgs a)
 
 			if (want == 8 * q + k)
 				p -= 1.0f;
-			x[q][k] = target >= 0 && inside ? p * a.scale : 0.0f;
+			x[q][k] = target >= 0 && inside ? p : 0.0f;
 		}
 		w.x = bf16_rne2(x[q].x, x[q].y);
 		w.y = bf16_rne2(x[q].z, x[q].w);
@@ -1009,6 +1011,7 @@ struct DxSumArgs {
 	int64_t		rows, rows_pad;
 	int		d, d_slot;
 	const int32_t	*target;	/* ts */
+	float		scale;
 	void		*dx;
 	int64_t		ld_dx;
 };
@@ -1024,24 +1027,25 @@ struct DwArgs {
 	int64_t		v0;
 	void		*dw;		/* [d][vocab] or NULL */
 	void		*db;		/* [vocab] or NULL */
+	float		scale;
 	int		splits;		/* slices of the tokens; more than one: into slots */
 	float		*slot;		/* [splits][slot_rows + 1][ld_slot], the last line for db */
 	int64_t		slot_rows, ld_slot;
 };
 
-/* base[i] += x */
+/* base[i] += scale x, rounded once */
 template <int GT>
-__device__ __forceinline__ void add_to(void *base, int64_t i, float x)
+__device__ __forceinline__ void add_to(void *base, int64_t i, float x, float scale)
 {
 	if constexpr (GT == kF32)
-		((float *)base)[i] += x;
+		((float *)base)[i] = __builtin_fmaf(scale, x, ((float *)base)[i]);
 	else
-		((uint16_t *)base)[i] = (uint16_t)bf16_rne(bf16_widen(((uint16_t *)base)[i]) + x);
+		((uint16_t *)base)[i] = (uint16_t)bf16_rne(__builtin_fmaf(scale, x, bf16_widen(((uint16_t *)base)[i])));
 }
 
 /* The same for the first n of N neighbours: all loads ahead of the stores, which the compiler cannot tell apart. */
 template <int GT, int N>
-__device__ __forceinline__ void add_some(void *base, int64_t i, int64_t n, const float *x)
+__device__ __forceinline__ void add_some(void *base, int64_t i, int64_t n, const float *x, float scale)
 {
 	float old[N];
 
@@ -1055,9 +1059,9 @@ __device__ __forceinline__ void add_some(void *base, int64_t i, int64_t n, const
 	for (int e = 0; e < N; e++)
 		if (e < n) {
 			if constexpr (GT == kF32)
-				((float *)base)[i + e] = old[e] + x[e];
+				((float *)base)[i + e] = __builtin_fmaf(scale, x[e], old[e]);
 			else
-				((uint16_t *)base)[i + e] = (uint16_t)bf16_rne(old[e] + x[e]);
+				((uint16_t *)base)[i + e] = (uint16_t)bf16_rne(__builtin_fmaf(scale, x[e], old[e]));
 		}
 }
 
@@ -1131,7 +1135,7 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 			const int64_t v = a.v0 + tv * SIDE + wn * (NB * 32) + j * 32 + lane;
 
 			if (v < a.vocab)
-				add_to<GT>(a.db, v, prod.sum[j][0]);
+				add_to<GT>(a.db, v, prod.sum[j][0], a.scale);
 		}
 	}
 	if (!a.dw)
@@ -1180,7 +1184,7 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 			if (k >= a.d || beyond == kWide)
 				continue;
 			if (!near) {
-				add_some<GT, kWide>(a.dw, k * a.vocab + v, left, x);
+				add_some<GT, kWide>(a.dw, k * a.vocab + v, left, x, a.scale);
 				continue;
 			}
 			if (beyond)
@@ -1188,12 +1192,12 @@ __global__ __launch_bounds__(SIDE == 256 ? 512 : 256, 2) void head_dw_kernel(DwA
 			if constexpr (GT == kF32) {
 #pragma unroll
 				for (int e = 0; e < 4; e++)
-					w[e] = __float_as_uint(__uint_as_float(w[e]) + x[e]);
+					w[e] = __float_as_uint(__builtin_fmaf(a.scale, x[e], __uint_as_float(w[e])));
 			} else {
 #pragma unroll
 				for (int e = 0; e < 4; e++)
-					w[e] = bf16_rne2(__uint_as_float(w[e] << 16) + x[2 * e],
-					    __uint_as_float(w[e] & 0xffff0000u) + x[2 * e + 1]);
+					w[e] = bf16_rne2(__builtin_fmaf(a.scale, x[2 * e], __uint_as_float(w[e] << 16)),
+					    __builtin_fmaf(a.scale, x[2 * e + 1], __uint_as_float(w[e] & 0xffff0000u)));
 			}
 			if (beyond == 0) {
 				*(u32x4_any *)(first + k * a.vocab * (16 / kWide)) = w;
@@ -1247,12 +1251,13 @@ struct DwSumArgs {
 	int64_t		slot_rows, ld_slot;
 	int		d, vocab;
 	int64_t		v0, count;	/* places of this piece */
+	float		scale;
 	void		*dw;
 	void		*db;
 };
 
 /*
-** dx = the slots' sum in order, in the caller's type.  A row without a target has delta 0, but its product
+** dx = scale times the slots' sum in order, in the caller's type.  A row without a target has delta 0, but its product
 ** with a w that is not finite is NaN: it gets its 0 here, and its slots are not read.
 */
 template <int GT>
@@ -1273,6 +1278,7 @@ __device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_
 #pragma unroll 8
 		for (int k = 0; k < splits; k++)
 			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_slot + c);
+		s *= a.scale;
 #pragma unroll
 		for (int j = 0; j < 4; j++)
 			if (c + j < a.d) {
@@ -1284,7 +1290,7 @@ __device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_
 	}
 }
 
-/* dw and db += the slots' sums in order: a line of dw (or db, the last) to a row of `across` workgroups. */
+/* dw and db += scale times the slots' sums in order: a line of dw (or db, the last) to a row of `across` workgroups. */
 template <int GT>
 __device__ __forceinline__ void dw_sum(const DwSumArgs &a, int64_t block, int64_t blocks)
 {
@@ -1303,7 +1309,7 @@ __device__ __forceinline__ void dw_sum(const DwSumArgs &a, int64_t block, int64_
 #pragma unroll 8
 		for (int k = 0; k < a.splits; k++)
 			s += p[(int64_t)k * (a.slot_rows + 1) * a.ld_slot];
-		add_to<GT>(last ? a.db : a.dw, last ? a.v0 + c : r * a.vocab + a.v0 + c, s);
+		add_to<GT>(last ? a.db : a.dw, last ? a.v0 + c : r * a.vocab + a.v0 + c, s, a.scale);
 	}
 }
 
@@ -1361,7 +1367,6 @@ static void delta_launch(hipStream_t st, const HeadPlan &p, const LogitArgs &l, 
 	a.kept_v = l.kept_v;
 	a.target = l.target;
 	a.lse = l.lse;
-	a.scale = l.scale;
 	a.vocab = vocab;
 	a.v0 = l.v0;
 	a.groups_v = here / 128;
@@ -1522,7 +1527,6 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		la.v0 = v0;
 		la.tiles_v = here / p.tile_v;
 		la.lse = lse;
-		la.scale = (float)j.scale;
 		la.delta = delta;
 		la.delta_low = low;
 		la.ld_delta = p.ld_delta;
@@ -1551,6 +1555,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 		wa.v0 = v0;
 		wa.dw = j.d_dw;
 		wa.db = j.d_db;
+		wa.scale = (float)j.scale;
 		wa.splits = p.splits_w;
 		wa.slot = (float *)(work + p.off_slot_w);
 		wa.slot_rows = p.slot_rows_w;
@@ -1597,6 +1602,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			sw.d = j.d;
 			sw.vocab = j.vocab;
 			sw.v0 = v0;
+			sw.scale = wa.scale;
 			sw.count = left < p.piece ? left : p.piece;
 			sw.dw = j.d_dw;
 			sw.db = j.d_db;
@@ -1610,6 +1616,7 @@ static int head_run(const anni_head_job &j, const HeadPlan &p, bool grad)
 			sx.d = j.d;
 			sx.d_slot = p.d_slot;
 			sx.target = ts;
+			sx.scale = wa.scale;
 			sx.dx = j.d_dx;
 			sx.ld_dx = j.ld_dx;
 		}
