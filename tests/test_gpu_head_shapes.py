@@ -26,7 +26,8 @@ GRADIENTS = [(rows, d, vocab, ty, pad) for rows, d, vocab, pad in [
     (16500, 24, 30000, BF16, 0.3),
     (2100, 499, 60001, F32, 0.3),   # and dw in large tiles, the logits kept or computed again
     (4097, 499, 66000, BF16, 0.3),
-]
+] + [(rows, d, vocab, ty, 0.2) for rows, d, vocab in [      # each axis at its end
+    (1 << 22, 1, 2), (5, 8, 1 << 22), (3, 1 << 16, 40), (262149, 24, 130)] for ty in (F32, BF16)]
 LOSSES = [(254, 64, 256, True), (777, 331, 10007, True), (517, 712, 50257, False), (1020, 257, 16381, False),
           (2040, 257, 16381, True), (1020, 512, 32768, False)]
 
