@@ -1078,8 +1078,9 @@ __device__ __forceinline__ u32x4 moved_down(u32x4 w, int halves)
 }
 
 /*
-** SIDE: of the tile both ways.  Few tokens leave little to contract and dw to read and write: smaller
-** tiles then, several workgroups to a compute unit, one at its products while others are at theirs.
+** SIDE: of the tile both ways.  Small tiles, several workgroups to a compute unit, where the large ones would leave
+** the chip idle; the rule (head_plan()) goes by the tiles and not by the tokens, so few tokens of a wide head
+** take the large ones, one workgroup to a compute unit, and wait for dw between their few steps.
 ** 96 tokens, 1536 x 100000 bf16: 170 us for 614 MB of dw in and out, 3.6 TB/s; non-temporal accesses and
 ** old values read ahead of the products were no faster.  4096 tokens: 610 us for half the
 ** vocabulary, 1030 TFLOP/s.
@@ -1257,8 +1258,9 @@ struct DwSumArgs {
 };
 
 /*
-** dx = scale times the slots' sum in order, in the caller's type.  A row without a target has delta 0, but its product
-** with a w that is not finite is NaN: it gets its 0 here, and its slots are not read.
+** dx = scale times the slots' sum in order, in the caller's type.  A row without a target has delta 0, but its
+** product with a w that is not finite is NaN: it gets its 0 here (the target and the slots are loaded together; one
+** behind the other 1 us more).
 */
 template <int GT>
 __device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_t blocks)
@@ -1273,12 +1275,12 @@ __device__ __forceinline__ void dx_sum(const DxSumArgs &a, int64_t block, int64_
 
 		if (c >= a.d)
 			continue;
-		const int splits = a.target[r] >= 0 ? a.splits : 0;
+		const bool live = a.target[r] >= 0;
 
 #pragma unroll 8
-		for (int k = 0; k < splits; k++)
+		for (int k = 0; k < a.splits; k++)
 			s += *(const f32x4 *)(a.slot + ((int64_t)k * a.rows_pad + r) * a.d_slot + c);
-		s *= a.scale;
+		s = live ? s * a.scale : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
 		for (int j = 0; j < 4; j++)
 			if (c + j < a.d) {
