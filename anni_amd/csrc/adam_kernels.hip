@@ -974,23 +974,6 @@ __global__ __launch_bounds__(kThreads) void adam_update_kernel(UpdateArgs a)
 	}
 }
 
-/* ---- the same update, software-pipelined (narrow storage modes) ----------------------- */
-
-/*
-** With bf16 moments or narrow gradients the update moves 22 - 28 bytes per element for the same
-** arithmetic (~90 vector instructions per element, 55 of them double precision), and it shows: a
-** wavefront that computes issues no memory instruction for thousands of cycles, and the memory
-** pipeline runs dry whenever all wavefronts of a SIMD compute (a kernel with the same nine
-** streams and no arithmetic is 9 % faster).  So here every wavefront has the loads of its NEXT tile in flight
-** while it computes the current one: two register stages of half a tile each, used in turn
-** (never copied -- a copy would wait for the loads it copies): while the first half of a tile is
-** computed its second half is on the way, while the second half is computed the first half of
-** the wavefront's next tile.  A stage holds the data as they lie in memory (16 + 8 + 8 + 8 bytes
-** per quad with bf16 storage) and is widened quad by quad when it is consumed.  Half-tile stages
-** need ~110 registers (whole-tile stages ~150) and were measured 0.6 % faster with fp8 gradients.
-** Arithmetic, rounding points and stores are those of adam_update_kernel; results are
-** bit-identical.
-*/
 /* ---- 8-bit moments ------------------------------------------------------------ */
 
 /*
@@ -1159,6 +1142,26 @@ __device__ __forceinline__ void tile_slow_q8(const UpdateArgs &a, const TileInfo
 		}
 	}
 }
+
+/* ---- the same update, software-pipelined (narrow storage modes) ----------------------- */
+
+/*
+** With bf16 moments or narrow gradients the update moves 22 - 28 bytes per element for the same
+** arithmetic (~90 vector instructions per element, 55 of them double precision), and it shows: a
+** wavefront that computes issues no memory instruction for thousands of cycles, and the memory
+** pipeline runs dry whenever all wavefronts of a SIMD compute (a kernel with the same nine
+** streams and no arithmetic is 9 % faster).  So here every wavefront has the loads of its NEXT tile in flight
+** while it computes the current one: two register stages of half a tile each, used in turn
+** (never copied -- a copy would wait for the loads it copies): while the first half of a tile is
+** computed its second half is on the way, while the second half is computed the first half of
+** the wavefront's next tile.  A stage holds the data as they lie in memory (16 + 8 + 8 + 8 bytes
+** per quad with bf16 storage) and is widened quad by quad when it is consumed.  Half-tile stages
+** need ~110 registers (whole-tile stages ~150) and were measured 0.6 % faster with fp8 gradients.
+** Arithmetic, rounding points and stores are those of adam_update_kernel; results are
+** bit-identical.  (8-bit moments, which that kernel does not have: whole tiles of one tensor take the step of
+** adam_step_near, the others the host loop's own, so which elements' p may be its neighbour follows the
+** tensors' places and the flats' alignment.)
+*/
 
 /* A tile that is skipped, ragged or shared by several tensors: as in adam_update_kernel. */
 template <int GT, int MT, bool NT, bool DER>

@@ -16,7 +16,7 @@
 ** pass turns logits into delta (bf16, in the work area, a piece of the vocabulary of at most 512 MiB
 ** at a time), which the other two products read.  The logits come from the first pass where the work
 ** area has room for them, 8 bytes of traffic for each, and are computed again where it has not: a third
-** more operations than the 6 rows d vocab that cannot be avoided (4096 tokens, 1536 x 100000: 1.41 +
+** more operations than the 6 rows d vocab that cannot be avoided (4096 tokens, 1536 x 100000: 1.39 +
 ** 0.38 ms against 1.20 + 1.38).  With float gradients delta is the sum of two bf16 numbers (16 bits
 ** of fraction, an error of 2^-17 against 2^-9), and the two products that read it run over both.
 **
@@ -27,8 +27,8 @@
 ** An operand lies in memory either with the contracted axis contiguous, or with its rows contiguous;
 ** the second kind is turned by the transposing LDS read, so nothing is transposed in memory.
 **
-** 4096 x 1536 x 100000 in bf16 runs at 1050 TFLOP/s in the first pass, 1090 in dx and 1030 in dw, where the
-** library's product of the same shape reaches 1090 (matrix pipes 69 % busy at 1.66 GHz; here 55 % at
+** 4096 x 1536 x 100000 in bf16 runs at 900 TFLOP/s in the first pass (1.39 ms; 1050 without the logits it writes), 1100
+** in dx and 1030 in dw, where the library's product of the same shape reaches 1090 (matrix pipes 69 % busy at 1.66 GHz; here 55 % at
 ** 2.05: the chip's power is what either runs into).
 */
 #include <hip/hip_runtime.h>
@@ -954,7 +954,7 @@ struct DxArgs {
 /*
 ** Each slice of the contracted axis (the vocabulary) has a slot of its own.  w's lines are the contiguous
 ** axis: 128 bytes of each per step.  4096 x 1536 x 50000 570 us, 1100 TFLOP/s; 96 x 1536 x 100000
-** 103 us for w's 307 MB.
+** 104 us for w's 307 MB.
 */
 template <class S>
 __global__ __launch_bounds__(S::threads) void head_dx_kernel(DxArgs a)
@@ -1081,7 +1081,7 @@ __device__ __forceinline__ u32x4 moved_down(u32x4 w, int halves)
 ** SIDE: of the tile both ways.  Small tiles, several workgroups to a compute unit, where the large ones would leave
 ** the chip idle; the rule (head_plan()) goes by the tiles and not by the tokens, so few tokens of a wide head
 ** take the large ones, one workgroup to a compute unit, and wait for dw between their few steps.
-** 96 tokens, 1536 x 100000 bf16: 170 us for 614 MB of dw in and out, 3.6 TB/s; non-temporal accesses and
+** 96 tokens, 1536 x 100000 bf16: 175 us for 614 MB of dw in and out, 3.5 TB/s; non-temporal accesses and
 ** old values read ahead of the products were no faster.  4096 tokens: 610 us for half the
 ** vocabulary, 1030 TFLOP/s.
 */

@@ -47,7 +47,8 @@ class HeadLoss:
         self._done(self.L.anni_head_loss(C.byref(j)))
 
     def run_on(self, opt, w_tensor, b_tensor, x, target, nll, scale=1.0, dx=None, ld_x=None, ld_dx=None):
-        """The same on an LmAdam's head: weights from its twins, gradients into its gradient flat (grad=False: none)."""
+        """The same on an LmAdam's head: weights from its twins, gradients into its gradient flat (grad=False: none);
+        dx in that flat's type."""
         if not self.grad and dx:
             raise ValueError("made for the loss alone")
         j = self._fill(x, target, nll, scale, dx, ld_x, ld_dx)

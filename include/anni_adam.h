@@ -50,7 +50,9 @@ extern "C" {
 ** hash of the element's index and t, so that averages as slow as beta2 = 0.999 still move (to
 ** nearest they would not: a step's change is less than half a code) and runs repeat bit for bit.
 ** The step on p is within 2^-43 of the host loop's quotient: the float that p becomes is its neighbour
-** in about one element of 10^8.
+** in about one element of 10^8.  (Whole tiles of 4096 elements inside one tensor; tiles that tensors share, and
+** all of them when the bound gradient flat does not begin at a multiple of four elements, take the host
+** loop's own division.  So those rare bits of p can differ between layouts; codes and exponents do not.)
 ** A positive v is stored as at least the smallest code.  A block that holds a value that is not
 ** finite reads as NaN as a whole (B = 255); skip_nonfinite keeps such gradients out.  Values below
 ** the smallest float (a block of v whose largest is under 2^-116) lose bits when they are read.
@@ -362,17 +364,20 @@ int	anni_colsum_add_batch(const anni_colsum *jobs, int n_jobs);
 ** [rows][ld_x] (the last hidden states), w the bf16 [d][vocab] matrix the step keeps as the twin of
 ** w_head (lang/lm.c's logits = h w_head + b_head), b float [vocab] or NULL.
 **   nll[i] = log sum_v exp(l[i][v]) - l[i][target_i]
-**   delta[i][v] = scale * (exp(l[i][v] - lse_i) - [v == target_i])
-**   dx = delta w^T (overwritten),  dw += x^T delta,  db += column sums of delta
+**   delta[i][v] = exp(l[i][v] - lse_i) - [v == target_i]
+**   dx = scale delta w^T (overwritten),  dw += scale x^T delta,  db += scale times delta's column sums
 ** dw and db are added to, so they can point straight into the gradient flat (what earlier
 ** microbatches left there stays; the step clears it); with scale = 1 / (B (T - 1)) they are the mean
 ** loss's.  A row whose target is not in [0, vocab) takes no part: its nll is 0, its dx 0, and
-** whatever its x holds reaches nothing.  A logit of -inf has probability 0; a row with nothing else
-** has no distribution: NaN.
+** whatever its x holds reaches nothing, also where w or b is not finite.  A logit of -inf has
+** probability 0; a row with nothing else has no distribution: NaN.
 **
 ** Sums are float, products of bf16 numbers exact.  delta is rounded to bf16 for ANNI_BF16 gradients
 ** and kept as a pair of bf16 numbers for ANNI_F32 (an error of 2^-17 of each element); db is summed
-** from the same numbers.  No atomics: a run repeats bit for bit.
+** from the same numbers.  scale, a float, multiplies the float sums and is in no rounding but the result's.
+** The exponentials are the hardware's: exp(a) is within (|a| + 2) 2^-23 of itself, and a logit and lse are
+** floats, so at logits of size L a probability is known to L 2^-23 of itself.  No atomics: a run repeats
+** bit for bit.
 **
 ** d_work: work_bytes of device memory, 256-byte aligned, at least anni_head_loss_work_bytes of the
 ** same sizes; nothing is kept in it between calls, and calls on different streams (or recorded
@@ -403,10 +408,10 @@ typedef struct anni_head_job {
 } anni_head_job;
 /*
 ** grad_type -1 (here only: a job that names it beside gradients is refused): the loss alone.  0 for sizes
-** or a type that are refused.  The first is the least; with
-** the second or more the logits of gradients stay in memory between the two passes (4 bytes for
-** each of rows * vocab, padded) instead of being computed again: the same bits sooner.  Up to 512
-** MiB of logits are part of the first as well; below a width of 192 the two are the same.
+** or a type that are refused.  The first is the least; with the second or more the logits of gradients
+** stay in memory between the two passes (4 bytes for each of rows * vocab, padded) instead of being
+** computed again: the same bits sooner.  Up to 512 MiB of logits are part of the first as well; below a
+** width of 192 the two are the same.
 */
 size_t	anni_head_loss_work_bytes(int64_t rows, int d, int vocab, int grad_type);
 size_t	anni_head_loss_work_bytes_keep(int64_t rows, int d, int vocab, int grad_type);
